@@ -49,6 +49,7 @@ extern "C" {
 #define EXL3B200_DTYPE_F16 0
 #define EXL3B200_DTYPE_BF16 1
 #define EXL3B200_DTYPE_F32 2
+#define EXL3B200_DTYPE_E4M3 3 /* paged caches only */
 
 /* flags of the matmul entry points */
 #define EXL3B200_FLAG_INPUT_ROTATED 1 /* x is already H128(x*suh)/sqrt(128) in fp16; suh unused */
@@ -541,6 +542,102 @@ EXL3B200_API int exl3b200_decode_layer_step(int rows, int rows_per_seq, int hidd
                                             void* v_cache, int max_ctx, const long long* pos, const float* inv_freq,
                                             float swiglu_limit, const exl3b200_peers* peers, void* state,
                                             size_t state_bytes, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * A paged key-value cache of one layer: k and v are [pages][page_size][kv_heads][head_dim]
+ * of one dtype (F16, BF16 or E4M3), both with the same strides (in elements; the last
+ * dimension is contiguous, every stride and both bases multiples of 16 bytes), so that any
+ * order of the other dimensions and slices of a wider pool serve.  head_dim 64 or 128.
+ * E4M3: the value of a stored x is x * k_scale[head] (v_scale[head]), device arrays of
+ * kv_heads fp32 or NULL for 1.  A slot is page * page_size + the offset in the page.  No
+ * counterpart in the reference, whose layers leave the cache to SGLang.
+ */
+typedef struct exl3b200_paged_cache {
+    void* k;
+    void* v;
+    int dtype;
+    int pages, page_size, kv_heads, head_dim;
+    long long page_stride, pos_stride, head_stride;
+    const float* k_scale;
+    const float* v_scale;
+} exl3b200_paged_cache;
+
+/*
+ * Append tokens to a paged cache with the position rotation (RoPE) applied on the way:
+ * for each token t < tokens, q_out[t] = R(positions[t]) q[t], and - when slots[t] >= 0 -
+ * k and v of the cache's slot slots[t] become R(positions[t]) k[t] and v[t].  R(p) turns
+ * pair i of a head's first `rotary` dims by the angle p * inv_freq[i]: (x, y) ->
+ * (x cos - y sin, y cos + x sin); the pair is dims (i, i + rotary/2), or with interleaved 1
+ * dims (2i, 2i + 1).  Angles are reduced in double precision.  E4M3: the stored value is
+ * rn(x / scale), saturated at 448.  Arithmetic in fp32, one rounding at the end.
+ *
+ * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] of in_dtype (F16,
+ * BF16 or F32) with token and head strides in elements; q_out of q_out_dtype (F16 or BF16;
+ * the cache's dtype unless that is E4M3); it may be q itself.  All bases and strides
+ * multiples of 16 bytes.  rotary: a multiple of 16 up to head_dim (0: no rotation).
+ * positions and slots: device int64 [tokens]; inv_freq device fp32 [rotary/2].  A negative
+ * slot (a padding row) leaves the cache as it is; one past the pool does too and records
+ * EXL3B200_EBADARG in the device status.  Slots of one call must differ.
+ */
+typedef struct exl3b200_rope_append_args {
+    exl3b200_paged_cache cache;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    const long long* positions;
+    const long long* slots;
+    const float* inv_freq;
+    long long q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    long long q_out_stride, q_out_head_stride;
+    int tokens, q_heads, rotary, interleaved;
+    int in_dtype, q_out_dtype;
+} exl3b200_rope_append_args;
+
+EXL3B200_API int exl3b200_rope_append(const exl3b200_rope_append_args* args, void* stream);
+
+/* most rows_per_seq * q_heads / kv_heads of exl3b200_paged_attention */
+#define EXL3B200_PAGED_MAX_ROWS 1024
+
+/*
+ * Attention of the newest rows_per_seq tokens of each sequence over its pages:
+ *   out[r, h] = sum_p softmax_p(s_p) v_p,  s_p = cap(scale * q[r, h] . k_p),
+ * row r = rows_per_seq * s + j is sequence s's token at position seq_lens[s] - rows_per_seq
+ * + j and sees the positions up to its own (causal), of those the last `window` when window
+ * is positive.  cap(x) = softcap * tanh(x / softcap), x when softcap is 0.  Position p of
+ * sequence s lies in page block_table[s][p / page_size]; entries that no row sees are not
+ * read.  A row that sees nothing (an empty sequence) gets zeros and lse -inf.  lse (may be
+ * NULL): fp32 [rows][q_heads], the natural logarithm of the sum of exp(s_p).
+ *
+ * q and out [seqs * rows_per_seq][q_heads][head_dim] of dtype F16 or BF16 (the cache's
+ * unless that is E4M3), row and head strides in elements, multiples of 8, 16-byte aligned
+ * bases.  block_table: device int32 [seqs][max_pages], row stride table_stride; seq_lens:
+ * device int32 [seqs], the new tokens included.  A length over max_pages * page_size is cut
+ * to it, a page id outside the pool reads as zeros; both record EXL3B200_EBADARG in the
+ * device status.  A NaN or infinity in v at a position that one row of a sequence sees may
+ * reach the sequence's other rows; beyond that nothing behind a mask is read.
+ *
+ * The sequences' lengths are read on the device: every CTA takes an equal run of the
+ * batch's 64- or 128-position units, and a second kernel joins the sequences that the runs
+ * cut, always in the same order.  scratch: exl3b200_paged_attention_scratch_size bytes,
+ * 256-byte aligned, no initialisation, per concurrent call.
+ */
+typedef struct exl3b200_paged_attention_args {
+    exl3b200_paged_cache cache;
+    const void* q;
+    void* out;
+    float* lse;
+    const int* block_table;
+    const int* seq_lens;
+    long long q_stride, q_head_stride, out_stride, out_head_stride, table_stride;
+    int seqs, rows_per_seq, q_heads, max_pages, window;
+    int dtype;
+    float scale, softcap;
+} exl3b200_paged_attention_args;
+
+EXL3B200_API size_t exl3b200_paged_attention_scratch_size(int rows_per_seq, int q_heads, int kv_heads, int head_dim);
+EXL3B200_API int exl3b200_paged_attention(const exl3b200_paged_attention_args* args, void* scratch,
+                                          size_t scratch_bytes, void* stream);
 
 /*
  * Checkpoint reader: copies count byte ranges of the open file fd (offsets[i],

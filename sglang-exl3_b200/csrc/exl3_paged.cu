@@ -1,0 +1,1030 @@
+// Paged key-value cache: the append of new tokens with the position rotation applied
+// on the way (exl3b200_rope_append), and the attention of a few new tokens per sequence
+// over its pages (exl3b200_paged_attention).
+//
+// A cache is [pages][page_size][kv_heads][head_dim] in any stride order whose last
+// dimension is contiguous, 16 bit or e4m3 with one fp32 scale per kv head.
+#include <climits>
+#include <cmath>
+
+#include <cuda_fp8.h>
+
+#include "exl3_common.cuh"
+#include "exl3_capi_internal.h"
+#include "exl3_grouped_dev.cuh"
+
+namespace exl3b200 {
+
+constexpr int kSms = 148;
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+
+enum PagedDtype { kF16 = EXL3B200_DTYPE_F16, kBf16 = EXL3B200_DTYPE_BF16, kF32 = EXL3B200_DTYPE_F32,
+                  kE4m3 = EXL3B200_DTYPE_E4M3 };
+
+struct AppendArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    unsigned char* k_cache;
+    unsigned char* v_cache;
+    const long long* positions;
+    const long long* slots;
+    const float* inv_freq;
+    const float* k_scale;
+    const float* v_scale;
+    int* status;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head;  // elements
+    long long c_page, c_pos, c_head;                                        // bytes
+    long long num_slots;
+    int tokens, q_heads, kv_heads, page_size, rotary;
+};
+
+constexpr int kAppThreads = 256;
+constexpr int kAppMaxTile = 4;   // tokens of a CTA
+constexpr int kAppMaxHalf = 64;  // rotated pairs of a head
+
+template <typename T> struct Vec8;  // eight values of an input row
+template <> struct Vec8<__half> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __half* p)
+    {
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p) : "memory");
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            f[2 * i] = t.x, f[2 * i + 1] = t.y;
+        }
+    }
+};
+template <> struct Vec8<__nv_bfloat16> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p)
+    {
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p) : "memory");
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    }
+};
+template <> struct Vec8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p)
+    {
+        asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "l"(p) : "memory");
+        asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "l"(p + 4) : "memory");
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    }
+};
+
+// two fp32 -> one packed pair, one rounding to nearest
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ void store8(void* p, const float (&f)[8])
+{
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()),
+                                              pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+}
+// e4m3, rounded to nearest even and saturated at 448 (a NaN stays one)
+__device__ __forceinline__ void store8_e4m3(void* p, const float (&f)[8], float scale)
+{
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_fp8x2_storage_t t = __nv_cvt_float2_to_fp8x2(
+            make_float2(__fdiv_rn(f[2 * i], scale), __fdiv_rn(f[2 * i + 1], scale)), __NV_SATFINITE, __NV_E4M3);
+        w[i >> 1] |= (uint32_t) t << (16 * (i & 1));
+    }
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+// One CTA: a tile of tokens, all their heads.  The tile's cosines and sines are computed
+// once into shared memory: the angle p * w_i (a position of up to 2^31 times an fp32
+// frequency) is a product of two doubles taken to a fraction of pi before it is rounded
+// to fp32, so that a far position turns by as exact an angle as a near one.  A thread
+// then takes 16-element units of a head: elements [a, a+8) and [b, b+8), whose pairs
+// turn together - half-split pairs (i, i + r/2) sit in the two vectors, adjacent pairs
+// inside each.  Units beyond the rotated part, and v, are copied.
+template <typename IN, typename QO, bool E4M3, int D>
+__global__ __launch_bounds__(kAppThreads) void exl3_rope_append_kernel(const __grid_constant__ AppendArgs a, int tile,
+                                                                       int interleaved)
+{
+    constexpr int kUnits = D / 16;                       // units of a head
+    constexpr int kHeadsPerPass = kAppThreads / kUnits;  // heads that the CTA takes at once
+    __shared__ float2 turn[kAppMaxTile][kAppMaxHalf];    // (cos, sin)
+    __shared__ long long at[kAppMaxTile];                // the token's byte offset in the cache, -1: not written
+    griddep_launch();
+    griddep_wait();
+    const int t0 = blockIdx.x * tile;
+    const int nt = min(tile, a.tokens - t0);
+    const int half = a.rotary >> 1;
+    for (int i = threadIdx.x; i < nt * half; i += kAppThreads) {
+        const int t = i / half, f = i - t * half;
+        const double x = (double) a.positions[t0 + t] * (double) a.inv_freq[f] * 0.31830988618379067154;
+        float s, c;
+        sincospif((float) (x - 2.0 * rint(x * 0.5)), &s, &c);
+        turn[t][f] = make_float2(c, s);
+    }
+    if (threadIdx.x < nt) {
+        const long long slot = a.slots[t0 + threadIdx.x];
+        long long off = -1;
+        if (slot >= a.num_slots) {
+            if (a.status) atomicCAS(a.status, 0, (int) kErrBadArgument);
+        } else if (slot >= 0) {
+            const long long page = slot / a.page_size;
+            off = page * a.c_page + (slot - page * a.page_size) * a.c_pos;
+        }
+        at[threadIdx.x] = off;
+    }
+    __syncthreads();
+    const int u = threadIdx.x % kUnits;
+    const bool rot_unit = 16 * u < a.rotary;
+    const bool split = rot_unit && !interleaved;
+    const int ea = split ? 8 * u : 16 * u, eb = split ? half + 8 * u : 16 * u + 8;
+    const int heads = a.q_heads + 2 * a.kv_heads;
+    int t = 0, h = threadIdx.x / kUnits;
+    while (h >= heads) h -= heads, ++t;
+    for (; t < nt;) {
+        const int kind = h < a.q_heads ? 0 : h < a.q_heads + a.kv_heads ? 1 : 2;  // q, k, v
+        const int hh = kind == 0 ? h : kind == 1 ? h - a.q_heads : h - a.q_heads - a.kv_heads;
+        const long long off = at[t];
+        if (kind == 0 || off >= 0) {
+            const long long tok = t0 + t;
+            const IN* src = kind == 0 ? reinterpret_cast<const IN*>(a.q) + tok * a.q_tok + hh * a.q_head
+                            : kind == 1 ? reinterpret_cast<const IN*>(a.k) + tok * a.k_tok + hh * a.k_head
+                                        : reinterpret_cast<const IN*>(a.v) + tok * a.v_tok + hh * a.v_head;
+            Vec8<IN> va, vb;
+            va.load(src + ea);
+            vb.load(src + eb);
+            float x[8], y[8];
+            va.get(x);
+            vb.get(y);
+            if (kind != 2 && rot_unit) {
+                const float2* cs = &turn[t][8 * u];
+                if (!interleaved) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 w = cs[i];
+                        const float p = x[i] * w.x - y[i] * w.y;
+                        y[i] = y[i] * w.x + x[i] * w.y;
+                        x[i] = p;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 w = cs[i], z = cs[i + 4];
+                        float p = x[2 * i] * w.x - x[2 * i + 1] * w.y;
+                        x[2 * i + 1] = x[2 * i + 1] * w.x + x[2 * i] * w.y;
+                        x[2 * i] = p;
+                        p = y[2 * i] * z.x - y[2 * i + 1] * z.y;
+                        y[2 * i + 1] = y[2 * i + 1] * z.x + y[2 * i] * z.y;
+                        y[2 * i] = p;
+                    }
+                }
+            }
+            if (kind == 0) {
+                QO* dst = reinterpret_cast<QO*>(a.q_out) + tok * a.qo_tok + hh * a.qo_head;
+                store8<QO>(dst + ea, x);
+                store8<QO>(dst + eb, y);
+            } else {
+                unsigned char* dst = (kind == 1 ? a.k_cache : a.v_cache) + off + hh * a.c_head;
+                if constexpr (E4M3) {
+                    const float* sp = kind == 1 ? a.k_scale : a.v_scale;
+                    const float sc = sp ? sp[hh] : 1.f;
+                    store8_e4m3(dst + ea, x, sc);
+                    store8_e4m3(dst + eb, y, sc);
+                } else {
+                    store8<QO>(dst + 2 * ea, x);
+                    store8<QO>(dst + 2 * eb, y);
+                }
+            }
+        }
+        h += kHeadsPerPass;
+        while (h >= heads) h -= heads, ++t;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+
+struct AttnArgs {
+    const void* q;
+    const unsigned char* k;
+    const unsigned char* v;
+    const int* table;
+    const int* lens;
+    const float* k_scale;
+    const float* v_scale;
+    void* out;
+    float* lse;
+    int4* desc;       // [ctas]: {sequence, head block, pieces, 0} of the split item that begins in the CTA's range
+    float* part_o;    // [2 ctas][mrows][D]: unnormalised partial outputs
+    float2* part_ml;  // [2 ctas][mrows]: their row maximum (base 2, less kRef) and sum
+    int* status;
+    long long q_row, q_head, out_row, out_head;  // elements
+    long long c_page, c_pos, c_head;             // bytes
+    long long table_row;
+    int seqs, rows, group, kv_heads, mblocks, mrows, mtotal;  // rows per sequence; m = row * group + head of the group
+    int max_pages, page_size, num_pages, capacity;
+    unsigned page_mul;
+    int page_sh1, page_sh2;
+    int window;
+    float scale, softcap;
+};
+
+constexpr int kAttnGroups = 4;  // position groups of a CTA: warps that share a unit of the cache
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                 "{%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                 "{%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void pg_ldsm4(uint32_t (&r)[4], unsigned s)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void pg_ldsm4t(uint32_t (&r)[4], unsigned s)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void pg_cp16(unsigned s, const void* g, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(g), "r"(bytes) : "memory");
+}
+// the two e4m3 values of a 16-bit half as an fp16 pair (exact)
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int hi)
+{
+    const unsigned short h = (unsigned short) (hi ? w >> 16 : w);
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
+    return r;
+}
+// weights as 16-bit hi + lo pairs: together about twice the type's significant bits, so
+// that rounding the weights costs nothing beside the rounding of the output
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, __nv_bfloat16)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack2(a - f.x, b - f.y, __nv_bfloat16());
+}
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, __half)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack2(a - f.x, b - f.y, __half());
+}
+
+// 2^x to 2 ulp, 0 for -inf
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+template <int D, bool F8> struct AttnShape {
+    static constexpr int kRowBytes = D * (F8 ? 1 : 2);
+    static constexpr int kChunks = kRowBytes / 16;           // 16-byte pieces of a row
+    static constexpr int kPos = F8 ? 32 : 16;                // positions of a warp's stage
+    static constexpr int kUnit = kAttnGroups * kPos;         // positions of a CTA's stage
+    static constexpr int kSlot = 2 * kPos * kRowBytes;       // bytes of K and V: 16 * D fp32 too
+    static_assert(kSlot == 16 * D * 4, "a stage holds a warp's partial output at the end of an item");
+    // 16-byte piece c of row r, so that eight rows of a piece column lie in distinct banks
+    static __device__ __forceinline__ int at(int r, int c)
+    {
+        const int x = kRowBytes >= 128 ? (r & 7) : ((r >> 1) & 3);
+        return r * kRowBytes + ((c ^ x) << 4);
+    }
+};
+
+// A position in the launch's sequence of units: (sequence, kv head and row block, unit of
+// the sequence's visible positions).  Every CTA owns a contiguous run of units.
+template <int UNIT> struct Walk {
+    int s, h, c, n, c0, lo, len;
+    __device__ __forceinline__ static int length(const AttnArgs& a, int s) { return min(max(__ldg(a.lens + s), 0), a.capacity); }
+    __device__ __forceinline__ void sequence(const AttnArgs& a)
+    {
+        len = length(a, s);
+        lo = a.window > 0 ? max(0, len - a.rows + 1 - a.window) : 0;
+        c0 = lo / UNIT;
+        n = max(1, (len + UNIT - 1) / UNIT - c0);  // a sequence without tokens has one (masked) unit: its rows are written too
+    }
+    __device__ __forceinline__ void next(const AttnArgs& a)
+    {
+        if (++c == n) {
+            c = 0;
+            if (++h == a.kv_heads * a.mblocks) {
+                h = 0;
+                if (++s < a.seqs) sequence(a);
+            }
+        }
+    }
+};
+
+// MW warps per position group: warp (pg, mw) takes rows 16 mw .. 16 mw + 15 of the item
+// and positions pg * kPos .. of each unit.
+template <int D, typename QT, bool F8, int MAXW>
+__global__ __launch_bounds__(32 * kAttnGroups * MAXW, MAXW == 1 ? 2 : 1)
+void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
+{
+    using S = AttnShape<D, F8>;
+    using MT = typename std::conditional<F8, __half, QT>::type;  // the MMAs' type
+    constexpr int kRef = std::is_same<MT, __half>::value ? 14 : 0;  // fp16 weights: up to 2^14, so that small ones keep their bits
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int sh_scan[kAttnGroups * MAXW];
+    __shared__ int sh_first[2];
+    __shared__ float sh_m[kAttnGroups][16 * MAXW], sh_l[kAttnGroups][16 * MAXW];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int mw_n = blockDim.x / (32 * kAttnGroups);
+    const int pg = warp / mw_n, mw = warp - pg * mw_n;
+    const int g = lane >> 2, c = lane & 3;
+    const int items = a.kv_heads * a.mblocks;  // of a sequence
+    const int ctas = gridDim.x;
+
+    // units of all sequences, and where this CTA's run begins
+    Walk<S::kUnit> w;
+    int u0, u1, total, grid;
+    {
+        const int per = (a.seqs + blockDim.x - 1) / blockDim.x;
+        const int s0 = min(a.seqs, tid * per), s1 = min(a.seqs, s0 + per);
+        int sum = 0;
+        for (int s = s0; s < s1; ++s) {
+            w.s = s;
+            w.sequence(a);
+            sum += w.n * items;
+            if (blockIdx.x == 0 && a.status && __ldg(a.lens + s) > a.capacity) atomicCAS(a.status, 0, (int) kErrBadArgument);
+        }
+        int inc = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int t = __shfl_up_sync(~0u, inc, d);
+            if (lane >= d) inc += t;
+        }
+        if (lane == 31) sh_scan[warp] = inc;
+        __syncthreads();
+        int before = 0;
+        total = 0;
+        for (int i = 0; i < (int) (blockDim.x >> 5); ++i) {
+            if (i < warp) before += sh_scan[i];
+            total += sh_scan[i];
+        }
+        grid = min(ctas, total);
+        u0 = (int) ((long long) blockIdx.x * total / grid);
+        u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
+        if ((int) blockIdx.x >= grid) {
+            if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+            return;
+        }
+        const int excl = before + inc - sum;
+        if (u0 >= excl && u0 < excl + sum) {
+            int at = excl, s = s0;
+            for (;; ++s) {
+                w.s = s;
+                w.sequence(a);
+                if (u0 < at + w.n * items) break;
+                at += w.n * items;
+            }
+            sh_first[0] = s;
+            sh_first[1] = u0 - at;
+        }
+        __syncthreads();
+        w.s = sh_first[0];
+        w.sequence(a);
+        w.h = sh_first[1] / w.n;
+        w.c = sh_first[1] - w.h * w.n;
+    }
+
+    const unsigned ring = (unsigned) __cvta_generic_to_shared(smem) + pg * (kStages * S::kSlot);
+    // rows of a stage, copied by the position group's warps; rows that no query row sees are zeroed
+    auto stage = [&](const Walk<S::kUnit>& x, int slot) {
+        const int p0 = (x.c0 + x.c) * S::kUnit + pg * S::kPos;
+        const int pos = p0 + (lane & (S::kPos - 1));
+        bool ok = pos >= x.lo && pos < x.len;
+        long long off = 0;
+        if (ok) {
+            const unsigned t = __umulhi(a.page_mul, (unsigned) pos);
+            const int pi = (int) ((t + (((unsigned) pos - t) >> a.page_sh1)) >> a.page_sh2);
+            const int page = __ldg(a.table + x.s * a.table_row + pi);
+            if ((unsigned) page >= (unsigned) a.num_pages) {
+                ok = false;
+                if (a.status) atomicCAS(a.status, 0, (int) kErrBadArgument);
+            } else {
+                off = page * a.c_page + (pos - pi * a.page_size) * a.c_pos + (x.h / a.mblocks) * a.c_head;
+            }
+        }
+        const unsigned valid = __ballot_sync(~0u, ok);
+        const unsigned base = ring + slot * S::kSlot;
+        constexpr int kRows = 32 / S::kChunks;  // rows of one warp-wide copy
+#pragma unroll
+        for (int i = 0; i < S::kPos / kRows; ++i) {
+            if (MAXW > 1 && i % mw_n != mw) continue;
+            const int row = i * kRows + lane / S::kChunks, ch = lane % S::kChunks;
+            const long long o = __shfl_sync(~0u, off, row) + ch * 16;
+            const int bytes = (valid >> row) & 1 ? 16 : 0;
+            const unsigned dst = base + S::at(row, ch);
+            pg_cp16(dst, a.k + o, bytes);
+            pg_cp16(dst + S::kPos * S::kRowBytes, a.v + o, bytes);
+        }
+    };
+    auto group_sync = [&] {
+        if (MAXW == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(pg + 1), "r"(32 * mw_n) : "memory");
+    };
+
+    // first stages
+    Walk<S::kUnit> f = w;  // runs ahead of w
+    int fu = u0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (fu < u1) {
+            stage(f, i);
+            f.next(a);
+            ++fu;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    uint32_t qf[D / 16][4];
+    float o[D / 8][4];
+    float rm[2], rl[2], rs[2];  // per row: running maximum (base 2), sum, and the scores' scale
+    int ve[2];                  // positions below are seen
+    int mbase = 0, mcount = 0;
+    int slot = 0;
+    bool fresh = true;
+    int item_u = u0;  // first unit of this CTA's piece of the item
+    for (int u = u0; u < u1; ++u) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        group_sync();
+        if (fu < u1) {
+            stage(f, slot == 0 ? kStages - 1 : slot - 1);
+            f.next(a);
+            ++fu;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (fresh) {  // a new item: its rows of q as A fragments
+            fresh = false;
+            item_u = u;
+            const int kvh = w.h / a.mblocks, mb = w.h - kvh * a.mblocks;
+            mbase = mb * a.mrows;
+            mcount = min(a.mrows, a.mtotal - mbase);
+            const float ks = (F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int m = 16 * mw + g + 8 * hf;
+                const int mm = mbase + min(m, mcount - 1);
+                const int j = mm / a.group;
+                const QT* qr = reinterpret_cast<const QT*>(a.q) + ((long long) w.s * a.rows + j) * a.q_row +
+                               (long long) (kvh * a.group + mm - j * a.group) * a.q_head;
+                ve[hf] = w.len - a.rows + 1 + j;  // (rows past the block's last repeat it and are not written)
+                rs[hf] = ks;
+                rm[hf] = -INFINITY;
+                rl[hf] = 0.f;
+                if constexpr (F8) {
+                    // e4m3 becomes fp16 exactly; a row of q in bf16 is taken into fp16's range by
+                    // a power of two that its scores' scale takes back.  k order of the MMA's
+                    // fragments: dims 4c .. 4c+3 of each 16, as four bytes of K come to a lane
+                    uint2 t[D / 16];
+                    float amax = 0.f;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) t[kk] = *reinterpret_cast<const uint2*>(qr + 16 * kk + 4 * c);
+                    if constexpr (std::is_same<QT, __half>::value) {
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) qf[kk][hf] = t[kk].x, qf[kk][2 + hf] = t[kk].y;
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[kk].x << 16)), fabsf(__uint_as_float(t[kk].x & 0xffff0000u))));
+                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[kk].y << 16)), fabsf(__uint_as_float(t[kk].y & 0xffff0000u))));
+                        }
+                        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+                        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+                        // amax * 2^-e in [2^13, 2^14); no scaling of zeros, infinities and NaN
+                        int e = (int) (__float_as_uint(amax) >> 23) - 127 - 13;
+                        if (amax == 0.f || !(amax < INFINITY)) e = 0;
+                        e = min(max(e, -100), 115);
+                        const float down = __uint_as_float((unsigned) (127 - e) << 23);
+                        rs[hf] = ks * __uint_as_float((unsigned) (127 + e) << 23);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            qf[kk][hf] = pack2(__uint_as_float(t[kk].x << 16) * down, __uint_as_float(t[kk].x & 0xffff0000u) * down, __half());
+                            qf[kk][2 + hf] = pack2(__uint_as_float(t[kk].y << 16) * down, __uint_as_float(t[kk].y & 0xffff0000u) * down, __half());
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        qf[kk][hf] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c);
+                        qf[kk][2 + hf] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * c);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        }
+
+        const int p0 = (w.c0 + w.c) * S::kUnit + pg * S::kPos;
+        const unsigned kb = ring + slot * S::kSlot, vb = kb + S::kPos * S::kRowBytes;
+#pragma unroll
+        for (int sb = 0; sb < S::kPos / 16; ++sb) {
+            const int ps = p0 + 16 * sb;
+            if (ps >= w.len || ps + 16 <= w.lo) continue;  // warp-uniform
+            // scores of 16 rows x 16 positions
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            if constexpr (F8) {
+#pragma unroll
+                for (int cc = 0; cc < S::kChunks; cc += 4)
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        uint32_t r[4];
+                        pg_ldsm4(r, kb + S::at(16 * sb + 8 * nt + (lane & 7), cc + (lane >> 3)));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma16816<MT>(s[nt], qf[cc + i], e4m3x2_f16x2(r[i], 0), e4m3x2_f16x2(r[i], 1));
+                    }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    uint32_t r[4];
+                    pg_ldsm4(r, kb + S::at((lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+                    mma16816<MT>(s[0], qf[kk], r[0], r[1]);
+                    mma16816<MT>(s[1], qf[kk], r[2], r[3]);
+                }
+            }
+            // scale, cap, mask
+            const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 &&
+                              (a.window <= 0 || ps >= w.len - a.window);
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int hf = i >> 1;
+                    float t = s[nt][i] * rs[hf];
+                    if (a.softcap > 0.f) t = a.softcap * tanhf(t / a.softcap);
+                    t *= kLog2e;
+                    if (!open) {
+                        const int pos = ps + 8 * nt + 2 * c + (i & 1);
+                        if (pos >= ve[hf] || (a.window > 0 && pos < ve[hf] - a.window)) t = -INFINITY;
+                    }
+                    s[nt][i] = t;
+                    mx[hf] = fmaxf(mx[hf], t);
+                }
+            float al[2], ref[2];
+            bool grew = false;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(~0u, mx[hf], 1));
+                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(~0u, mx[hf], 2));
+                const float mn = fmaxf(rm[hf], mx[hf]);
+                grew |= mn > rm[hf];
+                al[hf] = rm[hf] == -INFINITY ? 0.f : ex2(rm[hf] - mn);
+                rm[hf] = mn;
+                ref[hf] = mn == -INFINITY ? 0.f : mn - (float) kRef;
+            }
+            if (__any_sync(~0u, grew)) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) rl[hf] *= al[hf];
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    o[j][0] *= al[0], o[j][1] *= al[0];
+                    o[j][2] *= al[1], o[j][3] *= al[1];
+                }
+            }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const float x = ex2(s[nt][2 * hf] - ref[hf]), y = ex2(s[nt][2 * hf + 1] - ref[hf]);
+                    rl[hf] += x + y;
+                    split2(x, y, hi[2 * nt + hf], lo[2 * nt + hf], MT());
+                }
+            if constexpr (F8) {
+#pragma unroll
+                for (int jj = 0; jj < D / 32; ++jj) {
+                    uint32_t r[4];
+                    pg_ldsm4t(r, vb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * jj + (lane >> 4)));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {  // 16 dims: even ones in o[4 jj + 2 i], odd ones in the next
+                        const uint32_t ev = __byte_perm(r[2 * i], r[2 * i + 1], 0x6420);
+                        const uint32_t od = __byte_perm(r[2 * i], r[2 * i + 1], 0x7531);
+                        const uint32_t e0 = e4m3x2_f16x2(ev, 0), e1 = e4m3x2_f16x2(ev, 1);
+                        const uint32_t d0 = e4m3x2_f16x2(od, 0), d1 = e4m3x2_f16x2(od, 1);
+                        mma16816<MT>(o[4 * jj + 2 * i], hi, e0, e1);
+                        mma16816<MT>(o[4 * jj + 2 * i + 1], hi, d0, d1);
+                        mma16816<MT>(o[4 * jj + 2 * i], lo, e0, e1);
+                        mma16816<MT>(o[4 * jj + 2 * i + 1], lo, d0, d1);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    uint32_t r[4];
+                    pg_ldsm4t(r, vb + S::at((lane & 7) + (((lane >> 3) & 1) << 3), 2 * j + (lane >> 4)));
+                    mma16816<MT>(o[2 * j], hi, r[0], r[1]);
+                    mma16816<MT>(o[2 * j + 1], hi, r[2], r[3]);
+                    mma16816<MT>(o[2 * j], lo, r[0], r[1]);
+                    mma16816<MT>(o[2 * j + 1], lo, r[2], r[3]);
+                }
+            }
+        }
+
+        if (w.c == w.n - 1 || u == u1 - 1) {
+            // the end of the item's piece: join the position groups through the stage just read
+            group_sync();  // every warp of the group has read it
+            float* mine = mw == 0 ? reinterpret_cast<float*>(smem + pg * (kStages * S::kSlot) + slot * S::kSlot)
+                                  : reinterpret_cast<float*>(smem + kAttnGroups * kStages * S::kSlot +
+                                                             ((mw - 1) * kAttnGroups + pg) * S::kSlot);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                rl[hf] += __shfl_xor_sync(~0u, rl[hf], 1);
+                rl[hf] += __shfl_xor_sync(~0u, rl[hf], 2);
+                const int r = g + 8 * hf;
+                if (16 * mw + r < mcount) {
+                    if (c == 0) sh_m[pg][16 * mw + r] = rm[hf], sh_l[pg][16 * mw + r] = rl[hf];
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j)
+                            *reinterpret_cast<float4*>(mine + r * D + ((16 * j + 4 * c) ^ ((r & 7) * 8))) =
+                                make_float4(o[2 * j][2 * hf], o[2 * j + 1][2 * hf], o[2 * j][2 * hf + 1], o[2 * j + 1][2 * hf + 1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < D / 8; ++j)
+                            *reinterpret_cast<float2*>(mine + r * D + ((8 * j + 2 * c) ^ ((r & 7) * 8))) =
+                                make_float2(o[j][2 * hf], o[j][2 * hf + 1]);
+                    }
+                }
+            }
+            __syncthreads();
+            const bool whole = w.c == w.n - 1 && u - item_u == w.n - 1;
+            const bool starts = w.c == u - item_u;  // the piece holds the item's first unit
+            const int kvh = w.h / a.mblocks;
+            const long long part = 2ll * blockIdx.x + (starts ? 1 : 0);
+            const float vs = (F8 && a.v_scale) ? __ldg(a.v_scale + kvh) : 1.f;
+            constexpr int kVec = D / 4;  // threads of a row
+            for (int e = tid; e < mcount * kVec; e += blockDim.x) {
+                const int m = e / kVec, d = (e - m * kVec) * 4;
+                const int r = m & 15, mq = m >> 4;
+                float M = sh_m[0][m];
+#pragma unroll
+                for (int i = 1; i < kAttnGroups; ++i) M = fmaxf(M, sh_m[i][m]);
+                float L = 0.f;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < kAttnGroups; ++i) {
+                    const float mi = sh_m[i][m];
+                    const float k = mi == -INFINITY ? 0.f : ex2(mi - M);
+                    const float* src = mq == 0 ? reinterpret_cast<const float*>(smem + i * (kStages * S::kSlot) + slot * S::kSlot)
+                                               : reinterpret_cast<const float*>(smem + kAttnGroups * kStages * S::kSlot +
+                                                                                ((mq - 1) * kAttnGroups + i) * S::kSlot);
+                    const float4 t = *reinterpret_cast<const float4*>(src + r * D + (d ^ ((r & 7) * 8)));
+                    const float li = sh_l[i][m];
+                    if (mi != -INFINITY || li != 0.f) {  // (a group that saw only NaN: a sum, no maximum)
+                        const float kk = mi == -INFINITY ? 1.f : k;
+                        L += kk * li;
+                        y.x += kk * t.x, y.y += kk * t.y, y.z += kk * t.z, y.w += kk * t.w;
+                    }
+                }
+                if (whole) {
+                    const int mm = mbase + m, j = mm / a.group;
+                    const long long row = (long long) w.s * a.rows + j;
+                    const int head = kvh * a.group + mm - j * a.group;
+                    const float inv = L == 0.f ? 0.f : vs / L;
+                    QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + d;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv, QT()), pack2(y.z * inv, y.w * inv, QT()));
+                    if (a.lse && d == 0)
+                        a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
+                } else {
+                    *reinterpret_cast<float4*>(a.part_o + (part * a.mrows + m) * D + d) = y;
+                    if (d == 0) a.part_ml[part * a.mrows + m] = make_float2(M, L);
+                }
+            }
+            if (u == u1 - 1 && tid == 0) {
+                // a split item that begins here: how many CTAs hold it
+                int pieces = 0;
+                if (starts && !whole) {
+                    const long long last = (long long) u + (w.n - 1 - w.c);  // the item's last unit
+                    pieces = (int) (((last + 1) * grid - 1) / total) - (int) blockIdx.x + 1;
+                }
+                a.desc[blockIdx.x] = make_int4(w.s, w.h, pieces, 0);
+            }
+            __syncthreads();  // the stage may be filled again
+            fresh = true;
+        }
+        w.next(a);
+        slot = slot == kStages - 1 ? 0 : slot + 1;
+    }
+}
+
+// Joins the pieces of the items that the CTAs' runs split: block (x, y) takes the item that
+// begins in the run of CTA x and its rows 4y .. 4y + 3, a warp each, in the order of the
+// pieces (so that a result does not depend on timing).
+template <int D, typename QT, bool F8>
+__global__ __launch_bounds__(128) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
+{
+    constexpr int kRef = (F8 || std::is_same<QT, __half>::value) ? 14 : 0;
+    griddep_launch();
+    griddep_wait();
+    const int4 d = a.desc[blockIdx.x];
+    if (d.z == 0) return;
+    const int lane = threadIdx.x & 31;
+    const int m = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const int kvh = d.y / a.mblocks, mbase = (d.y - kvh * a.mblocks) * a.mrows;
+    if (m >= min(a.mrows, a.mtotal - mbase)) return;
+    auto piece = [&](int p) { return (p == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + p)) * a.mrows + m; };
+    constexpr int V = D / 32;
+    float M = -INFINITY;
+    for (int p = lane; p < d.z; p += 32) M = fmaxf(M, a.part_ml[piece(p)].x);
+#pragma unroll
+    for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
+    float L = 0.f, y[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = 0.f;
+    for (int p0 = 0; p0 < d.z; p0 += 32) {
+        float k = 0.f, l = 0.f;
+        if (p0 + lane < d.z) {
+            const float2 ml = a.part_ml[piece(p0 + lane)];
+            l = ml.y;
+            k = ml.x == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(ml.x - M);
+        }
+        L += k * l;
+        const int n = min(32, d.z - p0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float ki = __shfl_sync(~0u, k, i);
+            const float* src = a.part_o + piece(p0 + i) * D + lane * V;
+            float t[V];
+            if constexpr (V == 4) *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(src);
+            else *reinterpret_cast<float2*>(t) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] += ki * t[e];
+        }
+    }
+#pragma unroll
+    for (int i = 16; i; i >>= 1) L += __shfl_xor_sync(~0u, L, i);
+    const int mm = mbase + m, j = mm / a.group;
+    const long long row = (long long) d.x * a.rows + j;
+    const int head = kvh * a.group + mm - j * a.group;
+    const float vs = (F8 && a.v_scale) ? __ldg(a.v_scale + kvh) : 1.f;
+    const float inv = L == 0.f ? 0.f : vs / L;
+    QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + lane * V;
+#pragma unroll
+    for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2(y[e] * inv, y[e + 1] * inv, QT());
+    if (a.lse && lane == 0)
+        a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+template <typename Kern, typename... Args>
+static int paged_launch(Kern kern, dim3 grid, int block, int smem, cudaStream_t stream, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned) block);
+    cfg.dynamicSmemBytes = (size_t) smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+static bool misaligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
+// the strides of a cache, in bytes; false: a row would not begin on a 16-byte boundary
+static bool cache_strides(const exl3b200_paged_cache& c, long long* page, long long* pos, long long* head)
+{
+    const int e = c.dtype == kE4m3 ? 1 : 2;
+    *page = c.page_stride * e, *pos = c.pos_stride * e, *head = c.head_stride * e;
+    return !(misaligned(c.k, 16) || misaligned(c.v, 16) || *page % 16 || *pos % 16 || *head % 16);
+}
+
+static int check_cache(const exl3b200_paged_cache& c)
+{
+    if (!c.k || !c.v) return kErrNullPointer;
+    if (c.pages < 1 || c.page_size < 1 || c.kv_heads < 1 || (c.head_dim != 64 && c.head_dim != 128)) return kErrBadShape;
+    if (c.page_stride < 0 || c.pos_stride < 0 || c.head_stride < 0) return kErrBadShape;
+    if (c.dtype != kF16 && c.dtype != kBf16 && c.dtype != kE4m3) return kErrBadArgument;
+    return kOk;
+}
+
+template <typename IN, typename QO, bool E4M3>
+static int append_launch(const AppendArgs& a, int head_dim, int tile, int interleaved, cudaStream_t st)
+{
+    const dim3 grid((unsigned) ((a.tokens + tile - 1) / tile));
+    if (head_dim == 128) return paged_launch(exl3_rope_append_kernel<IN, QO, E4M3, 128>, grid, kAppThreads, 0, st, a, tile, interleaved);
+    return paged_launch(exl3_rope_append_kernel<IN, QO, E4M3, 64>, grid, kAppThreads, 0, st, a, tile, interleaved);
+}
+
+template <typename IN>
+static int append_types(const AppendArgs& a, int q_out, int cache, int head_dim, int tile, int interleaved, cudaStream_t st)
+{
+    if (cache == kE4m3)
+        return q_out == kF16 ? append_launch<IN, __half, true>(a, head_dim, tile, interleaved, st)
+                             : append_launch<IN, __nv_bfloat16, true>(a, head_dim, tile, interleaved, st);
+    return q_out == kF16 ? append_launch<IN, __half, false>(a, head_dim, tile, interleaved, st)
+                         : append_launch<IN, __nv_bfloat16, false>(a, head_dim, tile, interleaved, st);
+}
+
+template <int D, typename QT, bool F8, int MAXW>
+static int attn_launch(const AttnArgs& a, int ctas, int warps, cudaStream_t st)
+{
+    using S = AttnShape<D, F8>;
+    const int smem = kAttnGroups * S::kSlot * (kStages + warps - 1);
+    static bool done[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kErrLaunch;
+    auto kern = exl3_paged_attn_kernel<D, QT, F8, MAXW>;
+    if (!done[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kAttnGroups * S::kSlot * (kStages + MAXW - 1)) != cudaSuccess)
+            return kErrLaunch;
+        done[dev] = true;
+    }
+    const int rc = paged_launch(kern, dim3((unsigned) ctas), 32 * kAttnGroups * warps, smem, st, a);
+    if (rc != kOk) return rc;
+    return paged_launch(exl3_paged_join_kernel<D, QT, F8>, dim3((unsigned) ctas, (unsigned) ((a.mrows + 3) / 4)), 128, 0, st, a);
+}
+
+template <int D, typename QT, bool F8>
+static int attn_width(const AttnArgs& a, int ctas, int warps, cudaStream_t st)
+{
+    return warps == 1 ? attn_launch<D, QT, F8, 1>(a, ctas, warps, st) : attn_launch<D, QT, F8, 3>(a, ctas, warps, st);
+}
+
+template <typename QT>
+static int attn_types(const AttnArgs& a, int head_dim, bool f8, int ctas, int warps, cudaStream_t st)
+{
+    if (head_dim == 128) return f8 ? attn_width<128, QT, true>(a, ctas, warps, st) : attn_width<128, QT, false>(a, ctas, warps, st);
+    return f8 ? attn_width<64, QT, true>(a, ctas, warps, st) : attn_width<64, QT, false>(a, ctas, warps, st);
+}
+
+// How the rows of a (sequence, kv head) go into items: up to 48 at once (three warps of 16),
+// more in blocks of equal size.
+struct AttnSplit {
+    int mtotal, mblocks, mrows, warps, ctas;
+    size_t o_bytes, ml_bytes, desc_bytes;
+};
+static AttnSplit attn_split(int rows, int group, int head_dim)
+{
+    AttnSplit s;
+    s.mtotal = rows * group;
+    s.mblocks = (s.mtotal + 47) / 48;
+    s.mrows = (s.mtotal + s.mblocks - 1) / s.mblocks;
+    s.warps = (s.mrows + 15) / 16;
+    s.ctas = s.warps == 1 ? 2 * kSms : kSms;
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    s.o_bytes = up((size_t) 2 * s.ctas * s.mrows * head_dim * 4);
+    s.ml_bytes = up((size_t) 2 * s.ctas * s.mrows * 8);
+    s.desc_bytes = up((size_t) s.ctas * 16);
+    return s;
+}
+
+}  // namespace exl3b200
+
+using namespace exl3b200;
+
+extern "C" int exl3b200_rope_append(const exl3b200_rope_append_args* p, void* stream)
+{
+    if (!p) return kErrNullPointer;
+    const exl3b200_paged_cache& c = p->cache;
+    if (const int rc = check_cache(c)) return rc;
+    if (!p->q || !p->k || !p->v || !p->q_out || !p->positions || !p->slots || (p->rotary > 0 && !p->inv_freq)) return kErrNullPointer;
+    if (p->tokens < 1 || p->q_heads < 1 || p->rotary < 0 || p->rotary > c.head_dim || p->rotary % 16) return kErrBadShape;
+    if (p->in_dtype != kF16 && p->in_dtype != kBf16 && p->in_dtype != kF32) return kErrBadArgument;
+    if (p->q_out_dtype != kF16 && p->q_out_dtype != kBf16) return kErrBadArgument;
+    if (c.dtype != kE4m3 && c.dtype != p->q_out_dtype) return kErrBadArgument;
+    if (p->interleaved != 0 && p->interleaved != 1) return kErrBadArgument;
+    const long long vec = p->in_dtype == kF32 ? 4 : 8;  // elements of 16 bytes
+    const long long in[] = {p->q_stride, p->q_head_stride, p->k_stride, p->k_head_stride, p->v_stride, p->v_head_stride};
+    for (long long s : in)
+        if (s % vec) return kErrUnaligned;
+    if (p->q_out_stride % 8 || p->q_out_head_stride % 8) return kErrUnaligned;
+    if (misaligned(p->q, 16) || misaligned(p->k, 16) || misaligned(p->v, 16) || misaligned(p->q_out, 16)) return kErrUnaligned;
+    AppendArgs a = {};
+    if (!cache_strides(c, &a.c_page, &a.c_pos, &a.c_head)) return kErrUnaligned;
+    a.q = p->q, a.k = p->k, a.v = p->v, a.q_out = p->q_out;
+    a.k_cache = reinterpret_cast<unsigned char*>(c.k), a.v_cache = reinterpret_cast<unsigned char*>(c.v);
+    a.positions = p->positions, a.slots = p->slots, a.inv_freq = p->inv_freq;
+    a.k_scale = c.k_scale, a.v_scale = c.v_scale;
+    a.q_tok = p->q_stride, a.q_head = p->q_head_stride, a.k_tok = p->k_stride, a.k_head = p->k_head_stride;
+    a.v_tok = p->v_stride, a.v_head = p->v_head_stride, a.qo_tok = p->q_out_stride, a.qo_head = p->q_out_head_stride;
+    a.num_slots = (long long) c.pages * c.page_size;
+    a.tokens = p->tokens, a.q_heads = p->q_heads, a.kv_heads = c.kv_heads, a.page_size = c.page_size, a.rotary = p->rotary;
+    a.status = exl3_status_dev_ptr();
+    if (!a.status) return kErrLaunch;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int tile = p->tokens >= 8 * kSms * kAppMaxTile ? kAppMaxTile : 1;
+    if (p->in_dtype == kF16) return append_types<__half>(a, p->q_out_dtype, c.dtype, c.head_dim, tile, p->interleaved, st);
+    if (p->in_dtype == kBf16) return append_types<__nv_bfloat16>(a, p->q_out_dtype, c.dtype, c.head_dim, tile, p->interleaved, st);
+    return append_types<float>(a, p->q_out_dtype, c.dtype, c.head_dim, tile, p->interleaved, st);
+}
+
+extern "C" size_t exl3b200_paged_attention_scratch_size(int rows_per_seq, int q_heads, int kv_heads, int head_dim)
+{
+    if (rows_per_seq < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+    if ((long long) rows_per_seq * (q_heads / kv_heads) > EXL3B200_PAGED_MAX_ROWS) return 0;
+    const AttnSplit s = attn_split(rows_per_seq, q_heads / kv_heads, head_dim);
+    return s.o_bytes + s.ml_bytes + s.desc_bytes;
+}
+
+extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, void* scratch, size_t scratch_bytes, void* stream)
+{
+    if (!p) return kErrNullPointer;
+    const exl3b200_paged_cache& c = p->cache;
+    if (const int rc = check_cache(c)) return rc;
+    if (!p->q || !p->out || !p->block_table || !p->seq_lens || !scratch) return kErrNullPointer;
+    if (p->seqs < 1 || p->max_pages < 1 || p->table_stride < p->max_pages || p->window < 0) return kErrBadShape;
+    const size_t need = exl3b200_paged_attention_scratch_size(p->rows_per_seq, p->q_heads, c.kv_heads, c.head_dim);
+    if (need == 0) return kErrBadShape;
+    if (p->dtype != kF16 && p->dtype != kBf16) return kErrBadArgument;
+    if (c.dtype != kE4m3 && c.dtype != p->dtype) return kErrBadArgument;
+    if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap) || !std::isfinite(p->scale)) return kErrBadArgument;
+    if (scratch_bytes < need) return kErrWorkspace;
+    if (misaligned(scratch, 256) || misaligned(p->q, 16) || misaligned(p->out, 16)) return kErrUnaligned;
+    if (p->q_stride % 8 || p->q_head_stride % 8 || p->out_stride % 8 || p->out_head_stride % 8) return kErrUnaligned;
+    AttnArgs a = {};
+    if (!cache_strides(c, &a.c_page, &a.c_pos, &a.c_head)) return kErrUnaligned;
+    const AttnSplit sp = attn_split(p->rows_per_seq, p->q_heads / c.kv_heads, c.head_dim);
+    // positions are 32-bit, and so is the number of units of a launch
+    const long long capacity = std::min((long long) p->max_pages * c.page_size, (long long) INT_MAX - 256);
+    if (((capacity + 63) / 64 + 1) * p->seqs * c.kv_heads * sp.mblocks > INT_MAX) return kErrBadShape;
+    a.q = p->q, a.out = p->out, a.lse = p->lse;
+    a.k = reinterpret_cast<const unsigned char*>(c.k), a.v = reinterpret_cast<const unsigned char*>(c.v);
+    a.table = p->block_table, a.lens = p->seq_lens, a.table_row = p->table_stride;
+    a.k_scale = c.k_scale, a.v_scale = c.v_scale;
+    unsigned char* w = reinterpret_cast<unsigned char*>(scratch);
+    a.part_o = reinterpret_cast<float*>(w);
+    a.part_ml = reinterpret_cast<float2*>(w + sp.o_bytes);
+    a.desc = reinterpret_cast<int4*>(w + sp.o_bytes + sp.ml_bytes);
+    a.q_row = p->q_stride, a.q_head = p->q_head_stride, a.out_row = p->out_stride, a.out_head = p->out_head_stride;
+    a.seqs = p->seqs, a.rows = p->rows_per_seq, a.group = p->q_heads / c.kv_heads, a.kv_heads = c.kv_heads;
+    a.mblocks = sp.mblocks, a.mrows = sp.mrows, a.mtotal = sp.mtotal;
+    a.max_pages = p->max_pages, a.page_size = c.page_size, a.num_pages = c.pages, a.capacity = (int) capacity;
+    // position / page_size as a multiplication (32-bit unsigned division by an invariant)
+    int l = 0;
+    while (l < 31 && (1u << l) < (unsigned) c.page_size) ++l;
+    a.page_mul = (unsigned) ((((1ull << l) - (unsigned) c.page_size) << 32) / (unsigned) c.page_size + 1);
+    a.page_sh1 = std::min(l, 1), a.page_sh2 = std::max(l - 1, 0);
+    a.window = p->window, a.scale = p->scale, a.softcap = p->softcap;
+    a.status = exl3_status_dev_ptr();
+    if (!a.status) return kErrLaunch;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const bool f8 = c.dtype == kE4m3;
+    return p->dtype == kF16 ? attn_types<__half>(a, c.head_dim, f8, sp.ctas, sp.warps, st)
+                            : attn_types<__nv_bfloat16>(a, c.head_dim, f8, sp.ctas, sp.warps, st);
+}

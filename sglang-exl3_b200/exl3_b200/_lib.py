@@ -29,11 +29,12 @@ STATUS_NAMES = {
 
 EBADSHAPE, EBADBITS, EBADCODEBOOK, EUNALIGNED, ELAUNCH, EWORKSPACE, ENULL, EBADARG, ETIMEOUT, EIO = range(1, 11)
 
-DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_E4M3 = 0, 1, 2, 3
 FLAG_INPUT_ROTATED = 1
 FLAG_SINGLE_CTA = 2
 FLAG_PAIR_CTA = 4
 GEMV_MAX_M = 16
+PAGED_MAX_ROWS = 1024
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -91,6 +92,34 @@ class Peers(ctypes.Structure):
 
 _f = ctypes.c_float
 
+
+class PagedCache(ctypes.Structure):
+    """``exl3b200_paged_cache``: one layer's paged key-value cache."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("dtype", _i), ("pages", _i), ("page_size", _i), ("kv_heads", _i),
+                ("head_dim", _i), ("page_stride", _ll), ("pos_stride", _ll), ("head_stride", _ll), ("k_scale", _vp),
+                ("v_scale", _vp)]
+
+
+class RopeAppendArgs(ctypes.Structure):
+    """``exl3b200_rope_append_args``: tokens rotated and appended to a paged cache."""
+
+    _fields_ = [("cache", PagedCache), ("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("positions", _vp),
+                ("slots", _vp), ("inv_freq", _vp), ("q_stride", _ll), ("q_head_stride", _ll), ("k_stride", _ll),
+                ("k_head_stride", _ll), ("v_stride", _ll), ("v_head_stride", _ll), ("q_out_stride", _ll),
+                ("q_out_head_stride", _ll), ("tokens", _i), ("q_heads", _i), ("rotary", _i), ("interleaved", _i),
+                ("in_dtype", _i), ("q_out_dtype", _i)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """``exl3b200_paged_attention_args``: the newest tokens of each sequence over its pages."""
+
+    _fields_ = [("cache", PagedCache), ("q", _vp), ("out", _vp), ("lse", _vp), ("block_table", _vp),
+                ("seq_lens", _vp), ("q_stride", _ll), ("q_head_stride", _ll), ("out_stride", _ll),
+                ("out_head_stride", _ll), ("table_stride", _ll), ("seqs", _i), ("rows_per_seq", _i), ("q_heads", _i),
+                ("max_pages", _i), ("window", _i), ("dtype", _i), ("scale", _f), ("softcap", _f)]
+
+
 # name -> (restype, argtypes); one entry per declaration in include/exl3_b200.h
 SIGNATURES = {
     "exl3b200_abi_version": (_i, []),
@@ -147,6 +176,9 @@ SIGNATURES = {
     "exl3b200_gemm_combine_scratch_size": (_sz, [_i, _i, _i]),
     "exl3b200_gemm_combine": (_i, [_vp, _ll, _i, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _ll, _vp, _vp, _i, _vp, _sz,
                                    _vp]),
+    "exl3b200_rope_append": (_i, [_vp, _vp]),
+    "exl3b200_paged_attention_scratch_size": (_sz, [_i, _i, _i, _i]),
+    "exl3b200_paged_attention": (_i, [_vp, _vp, _sz, _vp]),
     "exl3b200_read_ranges": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp, _sz, _i, _i, _vp]),
     "exl3b200_moe_state_size": (_sz, [_i, _i, _i, _i]),
     "exl3b200_moe_scratch_size": (_sz, [_i, _i, _i, _i]),
