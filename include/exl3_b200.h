@@ -639,6 +639,28 @@ EXL3B200_API size_t exl3b200_paged_attention_scratch_size(int rows_per_seq, int 
 EXL3B200_API int exl3b200_paged_attention(const exl3b200_paged_attention_args* args, void* scratch,
                                           size_t scratch_bytes, void* stream);
 
+/* most alternatives of exl3b200_token_logprobs */
+#define EXL3B200_LOGPROBS_MAX_TOP 32
+
+/*
+ * Log-probabilities under softmax(logits[r]), one pass over the logits:
+ *   logprob[r] = log p(tokens[r]) (-inf for an id outside [0, vocab)),
+ *   entropy[r] = -sum p log p in nats, and the `top` most likely tokens, most likely first
+ *   (equal logits: lower id first): top_ids and top_logprobs [rows][top].
+ * logits [rows][vocab] F16, BF16 or F32, row stride in elements, any element-aligned base;
+ * -inf marks excluded tokens (a row of nothing else, or one with a NaN or +inf, gives NaN).
+ * Sums in fp32.  tokens, top_ids: device int64; the other outputs fp32.  top 0..32, at most
+ * vocab; with 0 top_logprobs and top_ids may be NULL.  scratch:
+ * exl3b200_token_logprobs_scratch_size bytes (0: bad sizes), 16-byte aligned, no
+ * initialisation, per concurrent call.  No counterpart in the reference, whose callers take
+ * SGLang's sampler.
+ */
+EXL3B200_API size_t exl3b200_token_logprobs_scratch_size(int rows, int vocab, int top);
+EXL3B200_API int exl3b200_token_logprobs(const void* logits, long long row_stride, int rows, int vocab, int dtype,
+                                         const long long* tokens, int top, float* logprob, float* entropy,
+                                         float* top_logprobs, long long* top_ids, void* scratch,
+                                         size_t scratch_bytes, void* stream);
+
 /*
  * Checkpoint reader: copies count byte ranges of the open file fd (offsets[i],
  * sizes[i] bytes) to dst[i].  Replaces the pread() loop of the reference's

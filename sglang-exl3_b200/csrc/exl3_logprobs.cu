@@ -1,0 +1,507 @@
+// Log-probabilities of given tokens, the distribution's entropy and its top alternatives, in
+// one pass over the logits (exl3b200_token_logprobs).
+//
+//   lse = M + log sum_i exp(x_i - M)     logprob(t) = x_t - lse
+//   H   = lse - sum_i p_i x_i            = log S - T / S   with y_i = x_i - M,
+//                                          S = sum exp(y_i), T = sum y_i exp(y_i)
+//
+// in base 2 throughout (y = x log2(e) - M2).  Rows of 16-bit or fp32 logits are cut into
+// units of 256 vectors of 8 elements; every CTA takes an equal contiguous run of the units
+// of all rows, so that one row fills the machine as well as thousands do, and the pieces of
+// a row that lies in several runs are joined by a second kernel in a fixed order.
+//
+// Alternatives: each thread keeps the maximum of the vectors it saw and the vector that held
+// it, and the second largest vector maximum.  The k-th largest of the threads' maxima is a
+// lower bound of the k-th largest element; only the vectors of the k threads above it hold
+// candidates, and of those only the ones that the second maximum says so need to be read
+// again.  Elements are ordered by (value, lower index first) as unique 64-bit keys, so that
+// equal logits come in the order of their ids.
+#include <algorithm>
+#include <climits>
+
+#include "exl3_common.cuh"
+#include "exl3_capi_internal.h"
+#include "exl3_grouped_dev.cuh"
+
+namespace exl3b200 {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpVec = 8;                       // elements of a thread's vector
+constexpr int kLpUnit = kLpThreads * kLpVec;    // elements of a unit
+constexpr int kLpCtas = 4 * 148;
+constexpr int kLpMaxTop = EXL3B200_LOGPROBS_MAX_TOP;
+constexpr int kLpBuffer = 1024;                 // candidates kept before they are cut back to the best 32
+constexpr float kLpLog2e = 1.4426950408889634f;
+constexpr float kLpLn2 = 0.6931471805599453f;
+// The running reference of the exponents is raised only when an element exceeds it by 2^16:
+// sums of 2^31 terms below 2^16 stay far inside fp32.
+constexpr float kLpSlack = 16.f;
+
+typedef unsigned long long u64;
+
+struct LogprobArgs {
+    const void* logits;
+    const long long* tokens;
+    float* logprob;
+    float* entropy;
+    float* top_logprob;   // [rows][top]
+    long long* top_ids;   // [rows][top]
+    float4* part;         // [2 ctas]: {M, S, T, -} of a piece
+    u64* part_keys;       // [2 ctas][top]
+    long long row_stride;
+    int rows, vocab, top, row_units;
+};
+
+__device__ __forceinline__ float lp_ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// a lower bound on an exponent that lets a NaN through
+__device__ __forceinline__ float lp_bound(float y)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fC3480000;" : "=f"(r) : "f"(y));  // -200
+    return r;
+}
+// order of the values as unsigned integers (0 is below every value; -0 counts as 0)
+__device__ __forceinline__ unsigned lp_order(float x)
+{
+    const unsigned u = __float_as_uint(x + 0.f);
+    return u ^ ((unsigned) ((int) u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float lp_value(unsigned o)
+{
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ u64 lp_key(float x, int idx) { return (u64) lp_order(x) << 32 | (unsigned) ~idx; }
+__device__ __forceinline__ u64 lp_swap(u64 v, int j, bool larger)
+{
+    const u64 o = __shfl_xor_sync(~0u, v, j);
+    return (v > o) == larger ? v : o;
+}
+// a warp's 32 keys in descending order
+__device__ __forceinline__ u64 lp_sort(u64 v, int lane)
+{
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j; j >>= 1) v = lp_swap(v, j, ((lane & j) == 0) == ((lane & k) == 0));
+    return v;
+}
+// the 32 largest of two descending lists, descending
+__device__ __forceinline__ u64 lp_merge(u64 a, u64 b, int lane)
+{
+    const u64 r = __shfl_sync(~0u, b, 31 - lane);
+    u64 v = a > r ? a : r;
+#pragma unroll
+    for (int j = 16; j; j >>= 1) v = lp_swap(v, j, (lane & j) == 0);
+    return v;
+}
+// the 32 largest of every warp's list (descending), in warp 0
+__device__ __forceinline__ u64 lp_merge_warps(u64 v, u64 (*lists)[32], int warp, int lane)
+{
+#pragma unroll
+    for (int n = kLpWarps / 2; n; n >>= 1) {
+        if (warp >= n && warp < 2 * n) lists[warp][lane] = v;
+        __syncthreads();
+        if (warp < n) v = lp_merge(v, lists[warp + n][lane], lane);
+    }
+    return v;
+}
+
+// a vector's eight elements in fp32; elements outside the row are -inf
+template <typename T> __device__ __forceinline__ float lp_float(T x) { return (float) x; }
+template <> __device__ __forceinline__ float lp_float<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float lp_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T> struct LpVec {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                         : "l"(reinterpret_cast<const uint4*>(p) + i));
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i) {
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4) f[4 * i + j] = __uint_as_float(u[j]);
+                else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    f[2 * j] = __uint_as_float(u[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                } else {
+                    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+                    f[2 * j] = t.x, f[2 * j + 1] = t.y;
+                }
+            }
+        }
+    }
+};
+
+// A row as vectors that begin on 16-byte boundaries: vector 0 begins `shift` elements before
+// the row, the last one may end behind it; both are read element by element.
+template <typename T> struct LpRow {
+    const T* p;      // the row's first element, less shift
+    int shift, end;  // element e of the row is p[e + shift], e + shift < end
+    __device__ __forceinline__ LpRow(const LogprobArgs& a, int row)
+    {
+        const T* r = reinterpret_cast<const T*>(a.logits) + (long long) row * a.row_stride;
+        shift = (int) (((uintptr_t) r & 15) / sizeof(T));
+        p = r - shift;
+        end = shift + a.vocab;
+    }
+    __device__ __forceinline__ bool inside(int v) const { return v * kLpVec >= shift && (v + 1) * kLpVec <= end; }
+    __device__ __forceinline__ void edge(int v, float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = v * kLpVec + i;
+            f[i] = e >= shift && e < end ? lp_float<T>(p[e]) : -INFINITY;
+        }
+    }
+    __device__ __forceinline__ void read(int v, float (&f)[8]) const
+    {
+        if (inside(v)) {
+            LpVec<T> x;
+            x.load(p + v * kLpVec);
+            x.get(f);
+        } else {
+            edge(v, f);
+        }
+    }
+    __device__ __forceinline__ int vectors() const { return (end + kLpVec - 1) / kLpVec; }
+};
+
+// a finite logit for which (x - M) is taken instead of x log2 e - M2, whose product might overflow
+__device__ __forceinline__ bool lp_far(float M) { return fabsf(M) > 1e29f && fabsf(M) < INFINITY; }
+
+// A row's results from its maximum M, S and T (relative to M2 = M log2 e) and warp 0's
+// descending keys.
+template <typename T>
+__device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, float M, float S, float Tt, u64 key, int tid)
+{
+    const float M2 = M * kLpLog2e, ls = log2f(S);
+    auto of = [&](float x) { return lp_far(M) || lp_far(x) ? (x - M) - ls * kLpLn2 : (fmaf(x, kLpLog2e, -M2) - ls) * kLpLn2; };
+    if (tid == 0) {
+        const long long t = a.tokens[row];
+        float lp = -INFINITY;  // an id outside the vocabulary has no probability
+        if (t >= 0 && t < a.vocab) {
+            const float x = lp_float<T>(reinterpret_cast<const T*>(a.logits)[(long long) row * a.row_stride + t]);
+            lp = of(x);
+        }
+        a.logprob[row] = lp;
+        a.entropy[row] = (ls - Tt / S) * kLpLn2;
+    }
+    if (tid < a.top) {
+        a.top_logprob[(long long) row * a.top + tid] = of(lp_value((unsigned) (key >> 32)));
+        a.top_ids[(long long) row * a.top + tid] = (long long) (unsigned) ~(unsigned) key;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __grid_constant__ LogprobArgs a)
+{
+    __shared__ u64 lists[kLpWarps][32];
+    __shared__ u64 buffer[kLpBuffer + kLpThreads * kLpVec];
+    __shared__ float red[kLpWarps][3];
+    __shared__ u64 sh_bound;
+    __shared__ int sh_count, sh_cols, cols[kLpThreads];
+    __shared__ int best_vec[kLpThreads];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long total = (long long) a.rows * a.row_units;
+    int u = (int) (blockIdx.x * total / gridDim.x);
+    const int u_end = (int) ((blockIdx.x + 1) * total / gridDim.x);
+    while (u < u_end) {
+        const int row = u / a.row_units;
+        const int c0 = u - row * a.row_units, c1 = min(a.row_units, c0 + (u_end - u));  // units of the row: the piece
+        u += c1 - c0;
+        const LpRow<T> r(a, row);
+        const int nv = r.vectors();
+        const int v0 = c0 * kLpThreads + tid, v1 = min(nv, c1 * kLpThreads);  // vectors v0, v0 + 256, ... of this thread
+        float best = -INFINITY, second = -INFINITY, ref = -1e30f, s = 0.f, t = 0.f;
+        int bv = v0;
+        auto take = [&](const float (&f)[8], int v) {
+            const float cm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+            second = fmaxf(second, fminf(best, cm));
+            if (cm > best) {
+                best = cm;
+                bv = v;
+                const float c2 = cm * kLpLog2e;
+                if (c2 > ref + kLpSlack) {
+                    const float d = ref - c2, k = lp_ex2(d);
+                    t = (t + d * s) * k;
+                    s *= k;
+                    ref = c2;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // (a -inf gives y e = 0 through the bound)
+                const float y = lp_bound(fmaf(f[i], kLpLog2e, -ref));
+                const float e = lp_ex2(y);
+                s += e;
+                t = fmaf(y, e, t);
+            }
+        };
+        {
+            constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+            int v = v0;
+            if (v < v1 && !r.inside(v)) {
+                float f[8];
+                r.edge(v, f);
+                take(f, v);
+                v += kLpThreads;
+            }
+            for (; v + (kAhead - 1) * kLpThreads < v1 && r.inside(v + (kAhead - 1) * kLpThreads); v += kAhead * kLpThreads) {
+                LpVec<T> x[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) x[i].load(r.p + (long long) (v + i * kLpThreads) * kLpVec);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    float f[8];
+                    x[i].get(f);
+                    take(f, v + i * kLpThreads);
+                }
+            }
+            for (; v < v1; v += kLpThreads) {
+                float f[8];
+                r.read(v, f);
+                take(f, v);
+            }
+        }
+
+        // M, S, T of the piece
+        float M = best;
+#pragma unroll
+        for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
+        if (lane == 0) red[warp][0] = M;
+        if (tid == 0) sh_count = sh_cols = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kLpWarps; ++i) M = fmaxf(M, red[i][0]);
+        if (lp_far(M)) {  // logits whose product with log2 e leaves fp32's exact range, as a mask of the type's lowest value
+            s = t = 0.f;
+            for (int v = v0; v < v1; v += kLpThreads) {
+                float f[8];
+                r.read(v, f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = lp_bound((f[i] - M) * kLpLog2e), e = lp_ex2(y);
+                    s += e;
+                    t = fmaf(y, e, t);
+                }
+            }
+        } else {
+            const float d = ref - M * kLpLog2e, k = s == 0.f ? 0.f : lp_ex2(d);
+            t = s == 0.f ? 0.f : (t + d * s) * k;
+            s *= k;
+        }
+        {
+#pragma unroll
+            for (int i = 16; i; i >>= 1) {
+                s += __shfl_xor_sync(~0u, s, i);
+                t += __shfl_xor_sync(~0u, t, i);
+            }
+            if (lane == 0) red[warp][1] = s, red[warp][2] = t;
+        }
+        u64 key = 0;
+        if (a.top > 0) {
+            float f[8];
+            if (v0 < v1) {
+                r.read(bv, f);
+#pragma unroll
+                for (int i = 7; i >= 0; --i) {
+                    const int e = bv * kLpVec + i;
+                    if (f[i] == best && e >= r.shift && e < r.end) key = lp_key(best, e - r.shift);
+                }
+            }
+            best_vec[tid] = bv;
+            const u64 mine = key;
+            key = lp_merge_warps(lp_sort(key, lane), lists, warp, lane);
+            if (a.top > 1) {
+                if (warp == 0 && lane == a.top - 1) sh_bound = key;
+                __syncthreads();
+                u64 bound = sh_bound;
+                auto push = [&](const float (&x)[8], int v) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = v * kLpVec + i;
+                        if (e >= r.shift && e < r.end) {
+                            const u64 k = lp_key(x[i], e - r.shift);
+                            if (k >= bound) buffer[atomicAdd(&sh_count, 1)] = k;
+                        }
+                    }
+                };
+                // the best vectors of the threads above the bound (at most 32 of them, unless
+                // the piece has fewer threads with elements than alternatives)
+                if (v0 < v1 && mine >= bound) {
+                    push(f, bv);
+                    if (v0 + kLpThreads < v1 && lp_order(second) >= (unsigned) (bound >> 32)) cols[atomicAdd(&sh_cols, 1)] = tid;
+                }
+                __syncthreads();
+                const int units = (v1 - c0 * kLpThreads + kLpThreads - 1) / kLpThreads;  // vectors of a column, at most
+                const int again = sh_cols * units;
+                for (int i0 = 0;; i0 += kLpThreads) {
+                    const int n = sh_count;
+                    __syncthreads();  // every thread has read it
+                    if (n > kLpBuffer) {  // cut back to the best 32, raise the bound
+                        if (warp == 0) {
+                            u64 l = 0;
+                            for (int b = 0; b < n; b += 32) l = lp_merge(l, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
+                            buffer[lane] = l;
+                            if (lane == a.top - 1) sh_bound = l;
+                            if (lane == 0) sh_count = 32;
+                        }
+                        __syncthreads();
+                        bound = sh_bound;
+                    }
+                    if (i0 >= again) break;
+                    if (i0 + tid < again) {
+                        const int col = cols[(i0 + tid) / units];
+                        const int v = c0 * kLpThreads + col + ((i0 + tid) % units) * kLpThreads;
+                        if (v < v1 && v != best_vec[col]) {
+                            float x[8];
+                            r.read(v, x);
+                            push(x, v);
+                        }
+                    }
+                    __syncthreads();
+                }
+                if (warp == 0) {
+                    key = 0;
+                    const int n = sh_count;
+                    for (int b = 0; b < n; b += 32) key = lp_merge(key, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
+                }
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+            float S = 0.f, Tt = 0.f;
+#pragma unroll
+            for (int i = 0; i < kLpWarps; ++i) S += red[i][1], Tt += red[i][2];
+            if (c1 - c0 == a.row_units) {
+                lp_write<T>(a, row, M, S, Tt, key, tid);
+            } else {
+                const int piece = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
+                if (lane == 0) a.part[piece] = make_float4(M, S, Tt, 0.f);
+                if (lane < a.top) a.part_keys[(long long) piece * a.top + lane] = key;
+            }
+        }
+        __syncthreads();  // shared memory is free for the next piece
+    }
+}
+
+// The row that begins in the run of CTA x of the first kernel and does not end there.
+template <typename T>
+__global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __grid_constant__ LogprobArgs a)
+{
+    __shared__ u64 lists[kLpWarps][32];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long total = (long long) a.rows * a.row_units;
+    const long long u0 = blockIdx.x * total / gridDim.x, u1 = (blockIdx.x + 1) * total / gridDim.x;
+    if (u0 == u1) return;
+    const int row = (int) ((u1 - 1) / a.row_units);  // the run's last row
+    const long long first = (long long) row * a.row_units, last = first + a.row_units - 1;
+    if (first < u0 || last < u1) return;  // began earlier, or ends here
+    const int pieces = (int) (((last + 1) * gridDim.x - 1) / total) - (int) blockIdx.x + 1;
+    auto at = [&](int p) { return p == 0 ? 2 * (int) blockIdx.x + 1 : 2 * ((int) blockIdx.x + p); };
+    float M = -INFINITY, S = 0.f, Tt = 0.f;
+    if (warp == 0) {
+        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, a.part[at(p)].x);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
+        for (int p = lane; p < pieces; p += 32) {
+            const float4 q = a.part[at(p)];
+            const float d = lp_far(M) ? (q.x - M) * kLpLog2e : q.x * kLpLog2e - M * kLpLog2e, k = lp_ex2(d);
+            S += q.y * k;
+            Tt += k == 0.f ? 0.f : (q.z + d * q.y) * k;
+        }
+#pragma unroll
+        for (int i = 16; i; i >>= 1) {
+            S += __shfl_xor_sync(~0u, S, i);
+            Tt += __shfl_xor_sync(~0u, Tt, i);
+        }
+    }
+    u64 key = 0;
+    if (a.top > 0) {
+        const int n = pieces * a.top;
+        for (int b = warp * 32; b < n; b += kLpThreads) {
+            const int i = b + lane;
+            u64 k = 0;
+            if (i < n) k = a.part_keys[(long long) at(i / a.top) * a.top + i % a.top];
+            key = lp_merge(key, lp_sort(k, lane), lane);
+        }
+        key = lp_merge_warps(key, lists, warp, lane);
+    }
+    if (warp == 0) lp_write<T>(a, row, M, S, Tt, key, tid);
+}
+
+static int lp_ctas(long long rows, int row_units) { return (int) std::min<long long>(kLpCtas, rows * row_units); }
+// (a row that does not begin on a 16-byte boundary reaches over one vector more)
+static int lp_row_units(int vocab) { return (int) (((long long) vocab + kLpVec - 1 + kLpUnit - 1) / kLpUnit); }
+
+template <typename T> static int lp_launch(const LogprobArgs& a, int ctas, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) ctas);
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, exl3_logprobs_kernel<T>, a) != cudaSuccess) return kErrLaunch;
+    if ((long long) a.rows * a.row_units % ctas == 0 && (long long) a.rows * a.row_units / ctas % a.row_units == 0) return kOk;  // no run cuts a row
+    return cudaLaunchKernelEx(&cfg, exl3_logprobs_join_kernel<T>, a) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+}  // namespace exl3b200
+
+using namespace exl3b200;
+
+extern "C" size_t exl3b200_token_logprobs_scratch_size(int rows, int vocab, int top)
+{
+    if (rows < 1 || vocab < 1 || vocab > (1 << 30) || top < 0 || top > kLpMaxTop || top > vocab) return 0;
+    const int units = lp_row_units(vocab);
+    if ((long long) rows * units > INT_MAX) return 0;
+    const size_t ctas = (size_t) lp_ctas(rows, units);
+    return 2 * ctas * (sizeof(float4) + (size_t) top * sizeof(u64));
+}
+
+extern "C" int exl3b200_token_logprobs(const void* logits, long long row_stride, int rows, int vocab, int dtype,
+                                       const long long* tokens, int top, float* logprob, float* entropy,
+                                       float* top_logprobs, long long* top_ids, void* scratch, size_t scratch_bytes,
+                                       void* stream)
+{
+    if (!logits || !tokens || !logprob || !entropy || !scratch || (top > 0 && (!top_logprobs || !top_ids))) return kErrNullPointer;
+    const size_t need = exl3b200_token_logprobs_scratch_size(rows, vocab, top);
+    if (need == 0 || (rows > 1 && row_stride < vocab)) return kErrBadShape;
+    if (dtype != EXL3B200_DTYPE_F16 && dtype != EXL3B200_DTYPE_BF16 && dtype != EXL3B200_DTYPE_F32) return kErrBadArgument;
+    if (scratch_bytes < need) return kErrWorkspace;
+    if ((uintptr_t) scratch % 16 || (uintptr_t) logits % (dtype == EXL3B200_DTYPE_F32 ? 4 : 2)) return kErrUnaligned;
+    LogprobArgs a = {};
+    a.logits = logits, a.tokens = tokens, a.logprob = logprob, a.entropy = entropy;
+    a.top_logprob = top_logprobs, a.top_ids = top_ids;
+    a.row_stride = row_stride, a.rows = rows, a.vocab = vocab, a.top = top, a.row_units = lp_row_units(vocab);
+    const int ctas = lp_ctas(rows, a.row_units);
+    a.part = reinterpret_cast<float4*>(scratch);
+    a.part_keys = reinterpret_cast<u64*>(a.part + 2 * ctas);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (dtype == EXL3B200_DTYPE_F16) return lp_launch<__half>(a, ctas, st);
+    if (dtype == EXL3B200_DTYPE_BF16) return lp_launch<__nv_bfloat16>(a, ctas, st);
+    return lp_launch<float>(a, ctas, st);
+}
