@@ -261,8 +261,10 @@ struct AttnArgs {
     float scale, softcap;
 };
 
-constexpr int kAttnGroups = 4;  // position groups of a CTA: warps that share a unit of the cache
+constexpr int kAttnWarps = 4;
 constexpr int kStages = 3;
+constexpr int kMaxTiles = 5;   // row tiles of 8 of an item
+constexpr int kItemRows = 8 * kMaxTiles;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -329,29 +331,45 @@ __device__ __forceinline__ float ex2(float x)
     return r;
 }
 
+// movmatrix: an 8x8 matrix of 16-bit elements, transposed across the warp
+__device__ __forceinline__ uint32_t pg_transpose(uint32_t x)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 template <int D, bool F8> struct AttnShape {
     static constexpr int kRowBytes = D * (F8 ? 1 : 2);
     static constexpr int kChunks = kRowBytes / 16;           // 16-byte pieces of a row
     static constexpr int kPos = F8 ? 32 : 16;                // positions of a warp's stage
-    static constexpr int kUnit = kAttnGroups * kPos;         // positions of a CTA's stage
-    static constexpr int kSlot = 2 * kPos * kRowBytes;       // bytes of K and V: 16 * D fp32 too
-    static_assert(kSlot == 16 * D * 4, "a stage holds a warp's partial output at the end of an item");
+    static constexpr int kUnit = kAttnWarps * kPos;          // positions of a CTA's stage
+    static constexpr int kSlot = 2 * kPos * kRowBytes;       // bytes of K and V
+    static constexpr int kQPitch = 2 * D + 16;               // bytes of a row of q in shared memory
+    static_assert(kSlot == 16 * D * 4, "a stage holds 16 rows of a warp's partial output at the end of an item");
     // 16-byte piece c of row r, so that eight rows of a piece column lie in distinct banks
     static __device__ __forceinline__ int at(int r, int c)
     {
         const int x = kRowBytes >= 128 ? (r & 7) : ((r >> 1) & 3);
         return r * kRowBytes + ((c ^ x) << 4);
     }
+    // q in shared memory (more than 16 rows) follows the ring
+    static constexpr int smem(int tiles) { return kAttnWarps * kStages * kSlot + (tiles > 2 ? 8 * tiles * kQPitch : 0); }
 };
 
 // A position in the launch's sequence of units: (sequence, kv head and row block, unit of
 // the sequence's visible positions).  Every CTA owns a contiguous run of units.
 template <int UNIT> struct Walk {
     int s, h, c, n, c0, lo, len;
-    __device__ __forceinline__ static int length(const AttnArgs& a, int s) { return min(max(__ldg(a.lens + s), 0), a.capacity); }
     __device__ __forceinline__ void sequence(const AttnArgs& a)
     {
-        len = length(a, s);
+        len = min(max(__ldg(a.lens + s), 0), a.capacity);
         lo = a.window > 0 ? max(0, len - a.rows + 1 - a.window) : 0;
         c0 = lo / UNIT;
         n = max(1, (len + UNIT - 1) / UNIT - c0);  // a sequence without tokens has one (masked) unit: its rows are written too
@@ -368,385 +386,458 @@ template <int UNIT> struct Walk {
     }
 };
 
-// MW warps per position group: warp (pg, mw) takes rows 16 mw .. 16 mw + 15 of the item
-// and positions pg * kPos .. of each unit.
-template <int D, typename QT, bool F8, int MAXW>
-__global__ __launch_bounds__(32 * kAttnGroups * MAXW, MAXW == 1 ? 2 : 1)
-void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
+// One CTA: its run of units, warp w the positions w * kPos .. of each, through a ring of
+// stages of its own (no barrier but at an item's end).  The cache is the MMAs' A operand and
+// the query rows (heads of the group, rows of the sequence) their N, so that 8 heads fill an
+// MMA without padding: S^T = K Q^T, its columns' running maxima and sums, the weights
+// transposed in registers (movmatrix) and O^T = V^T P^T.
+template <int D, typename QT, bool F8, int NT>
+__global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using S = AttnShape<D, F8>;
-    using MT = typename std::conditional<F8, __half, QT>::type;  // the MMAs' type
-    constexpr int kRef = std::is_same<MT, __half>::value ? 14 : 0;  // fp16 weights: up to 2^14, so that small ones keep their bits
+    using MT = typename std::conditional<F8, __half, QT>::type;      // the MMAs' type
+    constexpr int kRef = std::is_same<MT, __half>::value ? 14 : 0;   // fp16 weights: up to 2^14, so that small ones keep their bits
+    constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
+    constexpr bool kQShared = NT > 2;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int sh_scan[kAttnGroups * MAXW];
-    __shared__ int sh_first[2];
-    __shared__ float sh_m[kAttnGroups][16 * MAXW], sh_l[kAttnGroups][16 * MAXW];
+    __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
+    __shared__ float sh_rs[kRowScale ? 8 * NT : 1];
     griddep_launch();
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int mw_n = blockDim.x / (32 * kAttnGroups);
-    const int pg = warp / mw_n, mw = warp - pg * mw_n;
     const int g = lane >> 2, c = lane & 3;
     const int items = a.kv_heads * a.mblocks;  // of a sequence
-    const int ctas = gridDim.x;
 
-    // units of all sequences, and where this CTA's run begins
+    // units of all sequences, and where this CTA's run begins (every warp for itself)
     Walk<S::kUnit> w;
-    int u0, u1, total, grid;
-    {
-        const int per = (a.seqs + blockDim.x - 1) / blockDim.x;
-        const int s0 = min(a.seqs, tid * per), s1 = min(a.seqs, s0 + per);
-        int sum = 0;
-        for (int s = s0; s < s1; ++s) {
-            w.s = s;
+    int total = 0, grid, u0, u1;
+    for (w.s = lane; w.s < a.seqs; w.s += 32) {
+        w.sequence(a);
+        total += w.n * items;
+        if (blockIdx.x == 0 && warp == 0 && __ldg(a.lens + w.s) > a.capacity) atomicCAS(a.status, 0, (int) kErrBadArgument);
+    }
+    total = __reduce_add_sync(~0u, total);
+    grid = min((int) gridDim.x, total);
+    if ((int) blockIdx.x >= grid) {
+        if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    u0 = (int) ((long long) blockIdx.x * total / grid);
+    u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
+    for (int base = 0, s0 = 0;; s0 += 32) {
+        w.s = s0 + lane;
+        int n = 0;
+        if (w.s < a.seqs) {
             w.sequence(a);
-            sum += w.n * items;
-            if (blockIdx.x == 0 && a.status && __ldg(a.lens + s) > a.capacity) atomicCAS(a.status, 0, (int) kErrBadArgument);
+            n = w.n * items;
         }
-        int inc = sum;
+        int inc = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int t = __shfl_up_sync(~0u, inc, d);
             if (lane >= d) inc += t;
         }
-        if (lane == 31) sh_scan[warp] = inc;
-        __syncthreads();
-        int before = 0;
-        total = 0;
-        for (int i = 0; i < (int) (blockDim.x >> 5); ++i) {
-            if (i < warp) before += sh_scan[i];
-            total += sh_scan[i];
+        const unsigned past = __ballot_sync(~0u, u0 < base + inc);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            w.s = s0 + l;
+            const int in = u0 - base - __shfl_sync(~0u, inc - n, l);
+            w.sequence(a);
+            w.h = in / w.n;
+            w.c = in - w.h * w.n;
+            break;
         }
-        grid = min(ctas, total);
-        u0 = (int) ((long long) blockIdx.x * total / grid);
-        u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
-        if ((int) blockIdx.x >= grid) {
-            if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
-            return;
-        }
-        const int excl = before + inc - sum;
-        if (u0 >= excl && u0 < excl + sum) {
-            int at = excl, s = s0;
-            for (;; ++s) {
-                w.s = s;
-                w.sequence(a);
-                if (u0 < at + w.n * items) break;
-                at += w.n * items;
-            }
-            sh_first[0] = s;
-            sh_first[1] = u0 - at;
-        }
-        __syncthreads();
-        w.s = sh_first[0];
-        w.sequence(a);
-        w.h = sh_first[1] / w.n;
-        w.c = sh_first[1] - w.h * w.n;
+        base += __shfl_sync(~0u, inc, 31);
     }
 
-    const unsigned ring = (unsigned) __cvta_generic_to_shared(smem) + pg * (kStages * S::kSlot);
-    // rows of a stage, copied by the position group's warps; rows that no query row sees are zeroed
-    auto stage = [&](const Walk<S::kUnit>& x, int slot) {
-        const int p0 = (x.c0 + x.c) * S::kUnit + pg * S::kPos;
-        const int pos = p0 + (lane & (S::kPos - 1));
-        bool ok = pos >= x.lo && pos < x.len;
+    const unsigned ring = (unsigned) __cvta_generic_to_shared(smem) + warp * (kStages * S::kSlot);
+    const unsigned qsh = (unsigned) __cvta_generic_to_shared(smem) + kAttnWarps * kStages * S::kSlot;
+    // a lane's position in a stage, its index in the block table, and whether a query row may see it
+    auto locate = [&](const Walk<S::kUnit>& x, int& pos, int& pi) {
+        pos = (x.c0 + x.c) * S::kUnit + warp * S::kPos + (lane & (S::kPos - 1));
+        const unsigned t = __umulhi(a.page_mul, (unsigned) pos);
+        pi = (int) ((t + (((unsigned) pos - t) >> a.page_sh1)) >> a.page_sh2);
+        return pos >= x.lo && pos < x.len;
+    };
+    // its page, read a stage ahead of the stage's copies
+    auto page_of = [&](const Walk<S::kUnit>& x) {
+        int pos, pi;
+        return locate(x, pos, pi) ? __ldg(a.table + x.s * a.table_row + pi) : -1;
+    };
+    // the copies of a stage: 8 (or 4) lanes a row; rows that no query row sees are zeroed
+    auto stage = [&](const Walk<S::kUnit>& x, int slot, int page) {
+        int pos, pi;
+        bool ok = locate(x, pos, pi);
         long long off = 0;
         if (ok) {
-            const unsigned t = __umulhi(a.page_mul, (unsigned) pos);
-            const int pi = (int) ((t + (((unsigned) pos - t) >> a.page_sh1)) >> a.page_sh2);
-            const int page = __ldg(a.table + x.s * a.table_row + pi);
             if ((unsigned) page >= (unsigned) a.num_pages) {
                 ok = false;
-                if (a.status) atomicCAS(a.status, 0, (int) kErrBadArgument);
+                atomicCAS(a.status, 0, (int) kErrBadArgument);
             } else {
                 off = page * a.c_page + (pos - pi * a.page_size) * a.c_pos + (x.h / a.mblocks) * a.c_head;
             }
         }
         const unsigned valid = __ballot_sync(~0u, ok);
         const unsigned base = ring + slot * S::kSlot;
-        constexpr int kRows = 32 / S::kChunks;  // rows of one warp-wide copy
+        constexpr int kLanes = S::kChunks >= 8 ? 8 : S::kChunks;  // lanes of a row
+        constexpr int kRows = 32 / kLanes;
+        const int r0 = lane / kLanes, ch = lane % kLanes;
 #pragma unroll
         for (int i = 0; i < S::kPos / kRows; ++i) {
-            if (MAXW > 1 && i % mw_n != mw) continue;
-            const int row = i * kRows + lane / S::kChunks, ch = lane % S::kChunks;
+            const int row = i * kRows + r0;
             const long long o = __shfl_sync(~0u, off, row) + ch * 16;
             const int bytes = (valid >> row) & 1 ? 16 : 0;
             const unsigned dst = base + S::at(row, ch);
-            pg_cp16(dst, a.k + o, bytes);
-            pg_cp16(dst + S::kPos * S::kRowBytes, a.v + o, bytes);
+#pragma unroll
+            for (int x2 = 0; x2 < S::kChunks; x2 += kLanes) {
+                pg_cp16(dst + 16 * x2, a.k + o + 16 * x2, bytes);
+                pg_cp16(dst + 16 * x2 + S::kPos * S::kRowBytes, a.v + o + 16 * x2, bytes);
+            }
         }
-    };
-    auto group_sync = [&] {
-        if (MAXW == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(pg + 1), "r"(32 * mw_n) : "memory");
     };
 
     // first stages
     Walk<S::kUnit> f = w;  // runs ahead of w
     int fu = u0;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
+    int page = page_of(f);
+    auto fill = [&](int slot) {
         if (fu < u1) {
-            stage(f, i);
+            const Walk<S::kUnit> x = f;
             f.next(a);
-            ++fu;
+            const int next = ++fu < u1 ? page_of(f) : -1;
+            stage(x, slot, page);
+            page = next;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fill(i);
 
-    uint32_t qf[D / 16][4];
-    float o[D / 8][4];
-    float rm[2], rl[2], rs[2];  // per row: running maximum (base 2), sum, and the scores' scale
-    int ve[2];                  // positions below are seen
-    int mbase = 0, mcount = 0;
-    int slot = 0;
+    uint32_t qf[kQShared ? 1 : D / 16][NT][2];  // B fragments of q
+    float o[D / 16][NT][4];                     // O^T: dims g, g + 8 of a 16-dim tile x rows 2c, 2c + 1
+    float rm[NT][2], rl[NT][2];                 // rows 2c, 2c + 1 of a tile: running maximum (base 2), this lane's sum
+    float ks = 0.f;
+    int mbase = 0, mcount = 0, item_u = u0, slot = 0;
     bool fresh = true;
-    int item_u = u0;  // first unit of this CTA's piece of the item
     for (int u = u0; u < u1; ++u) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        group_sync();
-        if (fu < u1) {
-            stage(f, slot == 0 ? kStages - 1 : slot - 1);
-            f.next(a);
-            ++fu;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (fresh) {  // a new item: its rows of q as A fragments
+        __syncwarp();
+        fill(slot == 0 ? kStages - 1 : slot - 1);
+        if (fresh) {  // a new item: its rows of q
             fresh = false;
             item_u = u;
             const int kvh = w.h / a.mblocks, mb = w.h - kvh * a.mblocks;
             mbase = mb * a.mrows;
             mcount = min(a.mrows, a.mtotal - mbase);
-            const float ks = (F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale;
+            ks = (F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale;
+            // row m of the item (rows past its last repeat it and are not written)
+            auto q_row = [&](int m) {
+                const int mm = mbase + min(m, mcount - 1), j = mm / a.group;
+                return reinterpret_cast<const QT*>(a.q) + ((long long) w.s * a.rows + j) * a.q_row +
+                       (long long) (kvh * a.group + mm - j * a.group) * a.q_head;
+            };
+            // An e4m3 cache meets q in fp16, to which e4m3 converts exactly; a bf16 row is taken
+            // into fp16's range by a power of two that the scores' scale takes back.  Four bytes
+            // of a cache row come to a lane: dims 4c .. 4c + 3 of each 16 are its k slots.
+            auto power = [&](float amax, float* down) {
+                // amax 2^-e in [2^13, 2^14); zeros, infinities and NaN stay
+                int e = (int) (__float_as_uint(amax) >> 23) - 127 - 13;
+                if (amax == 0.f || !(amax < INFINITY)) e = 0;
+                e = min(max(e, -100), 115);
+                *down = __uint_as_float((unsigned) (127 - e) << 23);
+                return __uint_as_float((unsigned) (127 + e) << 23);
+            };
+            auto lo16 = [](uint32_t x) { return __uint_as_float(x << 16); };
+            auto hi16 = [](uint32_t x) { return __uint_as_float(x & 0xffff0000u); };
+            if constexpr (!kQShared) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int m = 16 * mw + g + 8 * hf;
-                const int mm = mbase + min(m, mcount - 1);
-                const int j = mm / a.group;
-                const QT* qr = reinterpret_cast<const QT*>(a.q) + ((long long) w.s * a.rows + j) * a.q_row +
-                               (long long) (kvh * a.group + mm - j * a.group) * a.q_head;
-                ve[hf] = w.len - a.rows + 1 + j;  // (rows past the block's last repeat it and are not written)
-                rs[hf] = ks;
-                rm[hf] = -INFINITY;
-                rl[hf] = 0.f;
-                if constexpr (F8) {
-                    // e4m3 becomes fp16 exactly; a row of q in bf16 is taken into fp16's range by
-                    // a power of two that its scores' scale takes back.  k order of the MMA's
-                    // fragments: dims 4c .. 4c+3 of each 16, as four bytes of K come to a lane
-                    uint2 t[D / 16];
-                    float amax = 0.f;
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) t[kk] = *reinterpret_cast<const uint2*>(qr + 16 * kk + 4 * c);
-                    if constexpr (std::is_same<QT, __half>::value) {
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) qf[kk][hf] = t[kk].x, qf[kk][2 + hf] = t[kk].y;
-                    } else {
+                for (int nt = 0; nt < NT; ++nt) {
+                    const QT* qr = q_row(8 * nt + g);
+                    if constexpr (!F8) {
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk) {
-                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[kk].x << 16)), fabsf(__uint_as_float(t[kk].x & 0xffff0000u))));
-                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[kk].y << 16)), fabsf(__uint_as_float(t[kk].y & 0xffff0000u))));
+                            qf[kk][nt][0] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c);
+                            qf[kk][nt][1] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * c);
                         }
-                        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-                        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-                        // amax * 2^-e in [2^13, 2^14); no scaling of zeros, infinities and NaN
-                        int e = (int) (__float_as_uint(amax) >> 23) - 127 - 13;
-                        if (amax == 0.f || !(amax < INFINITY)) e = 0;
-                        e = min(max(e, -100), 115);
-                        const float down = __uint_as_float((unsigned) (127 - e) << 23);
-                        rs[hf] = ks * __uint_as_float((unsigned) (127 + e) << 23);
+                    } else {
+                        float amax = 0.f;
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk) {
-                            qf[kk][hf] = pack2(__uint_as_float(t[kk].x << 16) * down, __uint_as_float(t[kk].x & 0xffff0000u) * down, __half());
-                            qf[kk][2 + hf] = pack2(__uint_as_float(t[kk].y << 16) * down, __uint_as_float(t[kk].y & 0xffff0000u) * down, __half());
+                            const uint2 t = *reinterpret_cast<const uint2*>(qr + 16 * kk + 4 * c);
+                            qf[kk][nt][0] = t.x, qf[kk][nt][1] = t.y;
+                            if constexpr (kRowScale)
+                                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(lo16(t.x)), fabsf(hi16(t.x))), fmaxf(fabsf(lo16(t.y)), fabsf(hi16(t.y)))));
+                        }
+                        if constexpr (kRowScale) {
+                            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+                            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+                            float down;
+                            const float up = power(amax, &down);
+                            if (warp == 0 && c == 0) sh_rs[8 * nt + g] = ks * up;
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+                                    qf[kk][nt][i] = pack2(lo16(qf[kk][nt][i]) * down, hi16(qf[kk][nt][i]) * down, __half());
                         }
                     }
-                } else {
+                }
+            } else {
+                // a warp a row: lane l holds dims of k slots in the order of the fragments
+                for (int m = warp; m < 8 * NT; m += kAttnWarps) {
+                    const QT* qr = q_row(m);
+                    constexpr int kPer = D / 32;  // dims of a lane, contiguous
+                    uint32_t t[kPer / 2];
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        qf[kk][hf] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c);
-                        qf[kk][2 + hf] = *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * c);
+                    for (int i = 0; i < kPer / 2; ++i) t[i] = *reinterpret_cast<const uint32_t*>(qr + kPer * lane + 2 * i);
+                    if constexpr (kRowScale) {
+                        float amax = 0.f;
+#pragma unroll
+                        for (int i = 0; i < kPer / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo16(t[i])), fabsf(hi16(t[i]))));
+#pragma unroll
+                        for (int i = 16; i; i >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, i));
+                        float down;
+                        const float up = power(amax, &down);
+                        if (lane == 0) sh_rs[m] = ks * up;
+#pragma unroll
+                        for (int i = 0; i < kPer / 2; ++i) t[i] = pack2(lo16(t[i]) * down, hi16(t[i]) * down, __half());
+                    }
+#pragma unroll
+                    for (int i = 0; i < kPer / 2; ++i) {
+                        const int d = kPer * lane + 2 * i;
+                        // e4m3: dims 4c, 4c + 1 of a 16 go to slots 2c, 2c + 1, dims 4c + 2, 4c + 3 to 8 + 2c, 9 + 2c
+                        const int at = F8 ? (d & ~15) + ((d & 2) ? 8 : 0) + ((d & 12) >> 1) : d;
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(qsh + m * S::kQPitch + 2 * at), "r"(t[i]) : "memory");
                     }
                 }
             }
+            if constexpr (kQShared || kRowScale) __syncthreads();
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) {
+                rm[nt][0] = rm[nt][1] = -INFINITY;
+                rl[nt][0] = rl[nt][1] = 0.f;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
+            }
         }
 
-        const int p0 = (w.c0 + w.c) * S::kUnit + pg * S::kPos;
+        const int p0 = (w.c0 + w.c) * S::kUnit + warp * S::kPos;
         const unsigned kb = ring + slot * S::kSlot, vb = kb + S::kPos * S::kRowBytes;
-#pragma unroll
+#pragma unroll 1
         for (int sb = 0; sb < S::kPos / 16; ++sb) {
             const int ps = p0 + 16 * sb;
             if (ps >= w.len || ps + 16 <= w.lo) continue;  // warp-uniform
-            // scores of 16 rows x 16 positions
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            if constexpr (F8) {
+            // scores: positions g, g + 8 x rows 2c, 2c + 1 of every tile
+            float s[NT][4];
 #pragma unroll
-                for (int cc = 0; cc < S::kChunks; cc += 4)
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile: a second chain of accumulations
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        uint32_t r[4];
-                        pg_ldsm4(r, kb + S::at(16 * sb + 8 * nt + (lane & 7), cc + (lane >> 3)));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma16816<MT>(s[nt], qf[cc + i], e4m3x2_f16x2(r[i], 0), e4m3x2_f16x2(r[i], 1));
-                    }
-            } else {
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
+            for (int kk = 0; kk < D / 16; kk += 2) {
+                uint32_t k0[4], k1[4];
+                if constexpr (F8) {
                     uint32_t r[4];
-                    pg_ldsm4(r, kb + S::at((lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-                    mma16816<MT>(s[0], qf[kk], r[0], r[1]);
-                    mma16816<MT>(s[1], qf[kk], r[2], r[3]);
+                    pg_ldsm4(r, kb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), kk + (lane >> 4)));
+                    k0[0] = e4m3x2_f16x2(r[0], 0), k0[1] = e4m3x2_f16x2(r[1], 0), k0[2] = e4m3x2_f16x2(r[0], 1), k0[3] = e4m3x2_f16x2(r[1], 1);
+                    k1[0] = e4m3x2_f16x2(r[2], 0), k1[1] = e4m3x2_f16x2(r[3], 0), k1[2] = e4m3x2_f16x2(r[2], 1), k1[3] = e4m3x2_f16x2(r[3], 1);
+                } else {
+                    const int row = (lane & 7) + (((lane >> 3) & 1) << 3);
+                    pg_ldsm4(k0, kb + S::at(row, 2 * kk + (lane >> 4)));
+                    pg_ldsm4(k1, kb + S::at(row, 2 * kk + 2 + (lane >> 4)));
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if constexpr (kQShared) {
+                        uint32_t r[4];
+                        pg_ldsm4(r, qsh + (8 * nt + (lane & 7)) * S::kQPitch + 32 * kk + 16 * (lane >> 3));
+                        mma16816<MT>(s[nt], k0, r[0], r[1]);
+                        mma16816<MT>(s[nt], k1, r[2], r[3]);
+                    } else {
+                        mma16816<MT>(s[nt], k0, qf[kk][nt][0], qf[kk][nt][1]);
+                        mma16816<MT>(NT == 1 ? s2 : s[nt], k1, qf[kk + 1][nt][0], qf[kk + 1][nt][1]);
+                    }
                 }
             }
-            // scale, cap, mask
-            const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 &&
-                              (a.window <= 0 || ps >= w.len - a.window);
-            float mx[2] = {-INFINITY, -INFINITY};
+            if (NT == 1)
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+                for (int i = 0; i < 4; ++i) s[0][i] += s2[i];
+            // scale, cap, mask; the tiles' maxima
+            const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 && (a.window <= 0 || ps >= w.len - a.window);
+            const float capl = a.softcap * kLog2e, icap = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
+            float mx[NT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int hf = i >> 1;
-                    float t = s[nt][i] * rs[hf];
-                    if (a.softcap > 0.f) t = a.softcap * tanhf(t / a.softcap);
-                    t *= kLog2e;
-                    if (!open) {
-                        const int pos = ps + 8 * nt + 2 * c + (i & 1);
-                        if (pos >= ve[hf] || (a.window > 0 && pos < ve[hf] - a.window)) t = -INFINITY;
-                    }
-                    s[nt][i] = t;
-                    mx[hf] = fmaxf(mx[hf], t);
+            for (int nt = 0; nt < NT; ++nt) {
+                float r0 = ks, r1 = ks;
+                if constexpr (kRowScale) {
+                    const float2 t = *reinterpret_cast<const float2*>(&sh_rs[8 * nt + 2 * c]);
+                    r0 = t.x, r1 = t.y;
                 }
-            float al[2], ref[2];
+                if (a.softcap > 0.f) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + exp(2 x / cap)))
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = ex2(s[nt][i] * ((i & 1) ? r1 : r0) * icap);
+                        s[nt][i] = fmaf(-2.f * capl, rcp(1.f + e), capl);
+                    }
+                } else {
+                    const float l0 = r0 * kLog2e, l1 = r1 * kLog2e;
+                    s[nt][0] *= l0, s[nt][1] *= l1, s[nt][2] *= l0, s[nt][3] *= l1;
+                }
+                if (!open) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int end = w.len - a.rows + 1 + (mbase + min(8 * nt + 2 * c + (i & 1), mcount - 1)) / a.group;
+                        const int pos = ps + g + 8 * (i >> 1);
+                        if (pos >= end || (a.window > 0 && pos < end - a.window)) s[nt][i] = -INFINITY;
+                    }
+                }
+                mx[nt][0] = fmaxf(s[nt][0], s[nt][2]);
+                mx[nt][1] = fmaxf(s[nt][1], s[nt][3]);
+            }
             bool grew = false;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(~0u, mx[hf], 1));
-                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(~0u, mx[hf], 2));
-                const float mn = fmaxf(rm[hf], mx[hf]);
-                grew |= mn > rm[hf];
-                al[hf] = rm[hf] == -INFINITY ? 0.f : ex2(rm[hf] - mn);
-                rm[hf] = mn;
-                ref[hf] = mn == -INFINITY ? 0.f : mn - (float) kRef;
-            }
-            if (__any_sync(~0u, grew)) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) rl[hf] *= al[hf];
+                for (int i = 0; i < 2; ++i) grew |= mx[nt][i] > rm[nt][i];
+            if (__any_sync(~0u, grew)) {  // some row's maximum rises
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    o[j][0] *= al[0], o[j][1] *= al[0];
-                    o[j][2] *= al[1], o[j][3] *= al[1];
+                for (int nt = 0; nt < NT; ++nt) {
+                    float al[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float x = mx[nt][i];
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                        x = fmaxf(x, rm[nt][i]);
+                        al[i] = rm[nt][i] == -INFINITY ? 0.f : ex2(rm[nt][i] - x);
+                        rm[nt][i] = x;
+                        rl[nt][i] *= al[i];
+                    }
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        o[j][nt][0] *= al[0], o[j][nt][1] *= al[1];
+                        o[j][nt][2] *= al[0], o[j][nt][3] *= al[1];
+                    }
                 }
             }
-            uint32_t hi[4], lo[4];
+            // weights, as B fragments (rows x positions) in hi + lo parts
+            uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                const float f0 = rm[nt][0] == -INFINITY ? 0.f : rm[nt][0] - (float) kRef;
+                const float f1 = rm[nt][1] == -INFINITY ? 0.f : rm[nt][1] - (float) kRef;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const float x = ex2(s[nt][2 * hf] - ref[hf]), y = ex2(s[nt][2 * hf + 1] - ref[hf]);
-                    rl[hf] += x + y;
-                    split2(x, y, hi[2 * nt + hf], lo[2 * nt + hf], MT());
+                    const float x = ex2(s[nt][2 * hf] - f0), y = ex2(s[nt][2 * hf + 1] - f1);
+                    rl[nt][0] += x;
+                    rl[nt][1] += y;
+                    split2(x, y, hi[nt][hf], lo[nt][hf], MT());
+                    hi[nt][hf] = pg_transpose(hi[nt][hf]);
+                    lo[nt][hf] = pg_transpose(lo[nt][hf]);
                 }
+            }
             if constexpr (F8) {
+                // 16 dims of V: rows g of the A fragment are dims 2g, rows g + 8 dims 2g + 1
 #pragma unroll
-                for (int jj = 0; jj < D / 32; ++jj) {
+                for (int j = 0; j < D / 16; j += 2) {
                     uint32_t r[4];
-                    pg_ldsm4t(r, vb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * jj + (lane >> 4)));
+                    pg_ldsm4t(r, vb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {  // 16 dims: even ones in o[4 jj + 2 i], odd ones in the next
+                    for (int i = 0; i < 2; ++i) {
                         const uint32_t ev = __byte_perm(r[2 * i], r[2 * i + 1], 0x6420);
                         const uint32_t od = __byte_perm(r[2 * i], r[2 * i + 1], 0x7531);
-                        const uint32_t e0 = e4m3x2_f16x2(ev, 0), e1 = e4m3x2_f16x2(ev, 1);
-                        const uint32_t d0 = e4m3x2_f16x2(od, 0), d1 = e4m3x2_f16x2(od, 1);
-                        mma16816<MT>(o[4 * jj + 2 * i], hi, e0, e1);
-                        mma16816<MT>(o[4 * jj + 2 * i + 1], hi, d0, d1);
-                        mma16816<MT>(o[4 * jj + 2 * i], lo, e0, e1);
-                        mma16816<MT>(o[4 * jj + 2 * i + 1], lo, d0, d1);
+                        const uint32_t v[4] = {e4m3x2_f16x2(ev, 0), e4m3x2_f16x2(od, 0), e4m3x2_f16x2(ev, 1), e4m3x2_f16x2(od, 1)};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[nt][0], hi[nt][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[nt][0], lo[nt][1]);
                     }
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
-                    uint32_t r[4];
-                    pg_ldsm4t(r, vb + S::at((lane & 7) + (((lane >> 3) & 1) << 3), 2 * j + (lane >> 4)));
-                    mma16816<MT>(o[2 * j], hi, r[0], r[1]);
-                    mma16816<MT>(o[2 * j + 1], hi, r[2], r[3]);
-                    mma16816<MT>(o[2 * j], lo, r[0], r[1]);
-                    mma16816<MT>(o[2 * j + 1], lo, r[2], r[3]);
+                    uint32_t v[4];
+                    pg_ldsm4t(v, vb + S::at((lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[nt][0], hi[nt][1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[nt][0], lo[nt][1]);
                 }
             }
         }
 
         if (w.c == w.n - 1 || u == u1 - 1) {
-            // the end of the item's piece: join the position groups through the stage just read
-            group_sync();  // every warp of the group has read it
-            float* mine = mw == 0 ? reinterpret_cast<float*>(smem + pg * (kStages * S::kSlot) + slot * S::kSlot)
-                                  : reinterpret_cast<float*>(smem + kAttnGroups * kStages * S::kSlot +
-                                                             ((mw - 1) * kAttnGroups + pg) * S::kSlot);
+            // the end of the item's piece: join the warps, 16 rows at a time, through the stage just read
+            float* mine = reinterpret_cast<float*>(smem + warp * (kStages * S::kSlot) + slot * S::kSlot);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                rl[hf] += __shfl_xor_sync(~0u, rl[hf], 1);
-                rl[hf] += __shfl_xor_sync(~0u, rl[hf], 2);
-                const int r = g + 8 * hf;
-                if (16 * mw + r < mcount) {
-                    if (c == 0) sh_m[pg][16 * mw + r] = rm[hf], sh_l[pg][16 * mw + r] = rl[hf];
-                    if constexpr (F8) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int j = 0; j < D / 16; ++j)
-                            *reinterpret_cast<float4*>(mine + r * D + ((16 * j + 4 * c) ^ ((r & 7) * 8))) =
-                                make_float4(o[2 * j][2 * hf], o[2 * j + 1][2 * hf], o[2 * j][2 * hf + 1], o[2 * j + 1][2 * hf + 1]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < D / 8; ++j)
-                            *reinterpret_cast<float2*>(mine + r * D + ((8 * j + 2 * c) ^ ((r & 7) * 8))) =
-                                make_float2(o[j][2 * hf], o[j][2 * hf + 1]);
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 4);
+                    rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 8);
+                    rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 16);
+                    if (g == 0) sh_m[warp][8 * nt + 2 * c + i] = rm[nt][i], sh_l[warp][8 * nt + 2 * c + i] = rl[nt][i];
                 }
-            }
-            __syncthreads();
             const bool whole = w.c == w.n - 1 && u - item_u == w.n - 1;
             const bool starts = w.c == u - item_u;  // the piece holds the item's first unit
             const int kvh = w.h / a.mblocks;
             const long long part = 2ll * blockIdx.x + (starts ? 1 : 0);
             const float vs = (F8 && a.v_scale) ? __ldg(a.v_scale + kvh) : 1.f;
-            constexpr int kVec = D / 4;  // threads of a row
-            for (int e = tid; e < mcount * kVec; e += blockDim.x) {
-                const int m = e / kVec, d = (e - m * kVec) * 4;
-                const int r = m & 15, mq = m >> 4;
-                float M = sh_m[0][m];
+            // element (r, d) of the 16 x D tile: d ^ 8 (r / 2 % 4), so that a warp's stores meet distinct banks
 #pragma unroll
-                for (int i = 1; i < kAttnGroups; ++i) M = fmaxf(M, sh_m[i][m]);
-                float L = 0.f;
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int n0 = 0; n0 < NT; n0 += 2) {
+                if (8 * n0 >= mcount) break;
+                __syncwarp();  // the stage has been read
 #pragma unroll
-                for (int i = 0; i < kAttnGroups; ++i) {
-                    const float mi = sh_m[i][m];
-                    const float k = mi == -INFINITY ? 0.f : ex2(mi - M);
-                    const float* src = mq == 0 ? reinterpret_cast<const float*>(smem + i * (kStages * S::kSlot) + slot * S::kSlot)
-                                               : reinterpret_cast<const float*>(smem + kAttnGroups * kStages * S::kSlot +
-                                                                                ((mq - 1) * kAttnGroups + i) * S::kSlot);
-                    const float4 t = *reinterpret_cast<const float4*>(src + r * D + (d ^ ((r & 7) * 8)));
-                    const float li = sh_l[i][m];
-                    if (mi != -INFINITY || li != 0.f) {  // (a group that saw only NaN: a sum, no maximum)
-                        const float kk = mi == -INFINITY ? 1.f : k;
-                        L += kk * li;
-                        y.x += kk * t.x, y.y += kk * t.y, y.z += kk * t.z, y.w += kk * t.w;
+                for (int nt = n0; nt < NT && nt < n0 + 2; ++nt)
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float* row = mine + (8 * (nt - n0) + 2 * c + i) * D;
+                            if constexpr (F8) {
+                                *reinterpret_cast<float2*>(row + ((16 * j + 2 * g) ^ (8 * c))) = make_float2(o[j][nt][i], o[j][nt][2 + i]);
+                            } else {
+                                row[(16 * j + g) ^ (8 * c)] = o[j][nt][i];
+                                row[(16 * j + 8 + g) ^ (8 * c)] = o[j][nt][2 + i];
+                            }
+                        }
+                __syncthreads();
+                constexpr int kVec = D / 4;  // threads of a row
+                for (int e = tid; e < min(16, mcount - 8 * n0) * kVec; e += 32 * kAttnWarps) {
+                    const int r = e / kVec, d = (e - r * kVec) * 4;
+                    const int m = 8 * n0 + r;
+                    float M = sh_m[0][m];
+#pragma unroll
+                    for (int i = 1; i < kAttnWarps; ++i) M = fmaxf(M, sh_m[i][m]);
+                    float L = 0.f;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < kAttnWarps; ++i) {
+                        const float mi = sh_m[i][m], li = sh_l[i][m];
+                        const float4 t = *reinterpret_cast<const float4*>(smem + i * (kStages * S::kSlot) + slot * S::kSlot +
+                                                                          4 * (r * D + (d ^ (8 * ((r >> 1) & 3)))));
+                        if (mi != -INFINITY || li != 0.f) {  // (a warp that saw only NaN: a sum, no maximum)
+                            const float k = mi == -INFINITY ? 1.f : ex2(mi - M);
+                            L += k * li;
+                            y.x += k * t.x, y.y += k * t.y, y.z += k * t.z, y.w += k * t.w;
+                        }
+                    }
+                    if (whole) {
+                        const int mm = mbase + m, j = mm / a.group;
+                        const long long row = (long long) w.s * a.rows + j;
+                        const int head = kvh * a.group + mm - j * a.group;
+                        const float inv = L == 0.f ? 0.f : vs / L;
+                        QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + d;
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv, QT()), pack2(y.z * inv, y.w * inv, QT()));
+                        if (a.lse && d == 0)
+                            a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
+                    } else {
+                        *reinterpret_cast<float4*>(a.part_o + (part * a.mrows + m) * D + d) = y;
+                        if (d == 0) a.part_ml[part * a.mrows + m] = make_float2(M, L);
                     }
                 }
-                if (whole) {
-                    const int mm = mbase + m, j = mm / a.group;
-                    const long long row = (long long) w.s * a.rows + j;
-                    const int head = kvh * a.group + mm - j * a.group;
-                    const float inv = L == 0.f ? 0.f : vs / L;
-                    QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + d;
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv, QT()), pack2(y.z * inv, y.w * inv, QT()));
-                    if (a.lse && d == 0)
-                        a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
-                } else {
-                    *reinterpret_cast<float4*>(a.part_o + (part * a.mrows + m) * D + d) = y;
-                    if (d == 0) a.part_ml[part * a.mrows + m] = make_float2(M, L);
-                }
+                __syncthreads();  // the stage may be filled again
             }
             if (u == u1 - 1 && tid == 0) {
                 // a split item that begins here: how many CTAs hold it
@@ -757,7 +848,6 @@ void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
                 }
                 a.desc[blockIdx.x] = make_int4(w.s, w.h, pieces, 0);
             }
-            __syncthreads();  // the stage may be filled again
             fresh = true;
         }
         w.next(a);
@@ -880,53 +970,53 @@ static int append_types(const AppendArgs& a, int q_out, int cache, int head_dim,
                          : append_launch<IN, __nv_bfloat16, false>(a, head_dim, tile, interleaved, st);
 }
 
-template <int D, typename QT, bool F8, int MAXW>
-static int attn_launch(const AttnArgs& a, int ctas, int warps, cudaStream_t st)
+template <int D, typename QT, bool F8, int NT>
+static int attn_launch(const AttnArgs& a, int ctas, cudaStream_t st)
 {
-    using S = AttnShape<D, F8>;
-    const int smem = kAttnGroups * S::kSlot * (kStages + warps - 1);
+    constexpr int smem = AttnShape<D, F8>::smem(NT);
     static bool done[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kErrLaunch;
-    auto kern = exl3_paged_attn_kernel<D, QT, F8, MAXW>;
+    auto kern = exl3_paged_attn_kernel<D, QT, F8, NT>;
     if (!done[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kAttnGroups * S::kSlot * (kStages + MAXW - 1)) != cudaSuccess)
-            return kErrLaunch;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrLaunch;
         done[dev] = true;
     }
-    const int rc = paged_launch(kern, dim3((unsigned) ctas), 32 * kAttnGroups * warps, smem, st, a);
+    const int rc = paged_launch(kern, dim3((unsigned) ctas), 32 * kAttnWarps, smem, st, a);
     if (rc != kOk) return rc;
     return paged_launch(exl3_paged_join_kernel<D, QT, F8>, dim3((unsigned) ctas, (unsigned) ((a.mrows + 3) / 4)), 128, 0, st, a);
 }
 
 template <int D, typename QT, bool F8>
-static int attn_width(const AttnArgs& a, int ctas, int warps, cudaStream_t st)
+static int attn_tiles(const AttnArgs& a, int ctas, cudaStream_t st)
 {
-    return warps == 1 ? attn_launch<D, QT, F8, 1>(a, ctas, warps, st) : attn_launch<D, QT, F8, 3>(a, ctas, warps, st);
+    const int tiles = (a.mrows + 7) / 8;
+    if (tiles == 1) return attn_launch<D, QT, F8, 1>(a, ctas, st);
+    if (tiles == 2) return attn_launch<D, QT, F8, 2>(a, ctas, st);
+    if (tiles == 3) return attn_launch<D, QT, F8, 3>(a, ctas, st);
+    return attn_launch<D, QT, F8, 5>(a, ctas, st);
 }
 
 template <typename QT>
-static int attn_types(const AttnArgs& a, int head_dim, bool f8, int ctas, int warps, cudaStream_t st)
+static int attn_types(const AttnArgs& a, int head_dim, bool f8, int ctas, cudaStream_t st)
 {
-    if (head_dim == 128) return f8 ? attn_width<128, QT, true>(a, ctas, warps, st) : attn_width<128, QT, false>(a, ctas, warps, st);
-    return f8 ? attn_width<64, QT, true>(a, ctas, warps, st) : attn_width<64, QT, false>(a, ctas, warps, st);
+    if (head_dim == 128) return f8 ? attn_tiles<128, QT, true>(a, ctas, st) : attn_tiles<128, QT, false>(a, ctas, st);
+    return f8 ? attn_tiles<64, QT, true>(a, ctas, st) : attn_tiles<64, QT, false>(a, ctas, st);
 }
 
-// How the rows of a (sequence, kv head) go into items: up to 48 at once (three warps of 16),
-// more in blocks of equal size.
+// How the rows of a (sequence, kv head) go into items: up to 40 at once, more in blocks of
+// equal size.
 struct AttnSplit {
-    int mtotal, mblocks, mrows, warps, ctas;
+    int mtotal, mblocks, mrows, ctas;
     size_t o_bytes, ml_bytes, desc_bytes;
 };
 static AttnSplit attn_split(int rows, int group, int head_dim)
 {
     AttnSplit s;
     s.mtotal = rows * group;
-    s.mblocks = (s.mtotal + 47) / 48;
+    s.mblocks = (s.mtotal + kItemRows - 1) / kItemRows;
     s.mrows = (s.mtotal + s.mblocks - 1) / s.mblocks;
-    s.warps = (s.mrows + 15) / 16;
-    s.ctas = s.warps == 1 ? 2 * kSms : kSms;
+    s.ctas = 2 * kSms;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     s.o_bytes = up((size_t) 2 * s.ctas * s.mrows * head_dim * 4);
     s.ml_bytes = up((size_t) 2 * s.ctas * s.mrows * 8);
@@ -1025,6 +1115,6 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     if (!a.status) return kErrLaunch;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool f8 = c.dtype == kE4m3;
-    return p->dtype == kF16 ? attn_types<__half>(a, c.head_dim, f8, sp.ctas, sp.warps, st)
-                            : attn_types<__nv_bfloat16>(a, c.head_dim, f8, sp.ctas, sp.warps, st);
+    return p->dtype == kF16 ? attn_types<__half>(a, c.head_dim, f8, sp.ctas, st)
+                            : attn_types<__nv_bfloat16>(a, c.head_dim, f8, sp.ctas, st);
 }

@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
+
+import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libexl3b200.so")
 
@@ -190,6 +193,12 @@ SIGNATURES = {
 }
 MULTI_MAX = 8
 
+# The argument structs of the calls whose host time shows, as one packed buffer each (the
+# native layout of the ctypes structures above, at a third of their construction's time).
+_CACHE_FORMAT = "PPiiiiiqqqPP"
+pack_rope_append = struct.Struct("@" + _CACHE_FORMAT + "PPPPPPPqqqqqqqqiiiiii").pack
+pack_paged_attention = struct.Struct("@" + _CACHE_FORMAT + "PPPPPqqqqqiiiiiiff").pack
+
 _lib = None
 _lock = threading.Lock()
 
@@ -225,3 +234,20 @@ def status_string(status: int) -> str:
 def check(status: int, what: str) -> None:
     if status != OK:
         raise RuntimeError(f"{what} failed: {status_string(status)} ({STATUS_NAMES.get(status, status)})")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(name: str, device: int, *args) -> None:
+    """Call an entry point on a device's current stream (the entry point's last argument);
+    raises on a status other than 0."""
+    fn = getattr(lib(), name)
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc != OK:
+        check(rc, name)

@@ -32,21 +32,21 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     top = int(top)
     if not 0 <= top <= min(_lib.LOGPROBS_MAX_TOP, vocab):
         raise RuntimeError(f"top must be 0..{_lib.LOGPROBS_MAX_TOP} and at most the vocabulary")
-    dev = _require_cuda(logits, tokens)
+    index = logits.get_device()
+    if index < 0 or tokens.get_device() != index:
+        _require_cuda(logits, tokens)
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     tokens = tokens.contiguous()
-    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    top_lp = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
+    dev = logits.device
+    got = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=dev),
+                        torch.empty(rows, dtype=torch.float32, device=dev),
+                        torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None,
+                        torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None)
     if rows:
-        L = _lib.lib()
-        n = L.exl3b200_token_logprobs_scratch_size(rows, vocab, top)
+        n = _lib.lib().exl3b200_token_logprobs_scratch_size(rows, vocab, top)
         scratch = torch.empty(n, dtype=torch.uint8, device=dev)  # the call's own (a captured graph keeps its own, too)
-        with torch.cuda.device(dev):
-            rc = L.exl3b200_token_logprobs(logits.data_ptr(), logits.stride(0), rows, vocab, _OUT_DTYPES[logits.dtype],
-                                           tokens.data_ptr(), top, both[0].data_ptr(), both[1].data_ptr(),
-                                           top_lp.data_ptr() if top else None, top_ids.data_ptr() if top else None,
-                                           scratch.data_ptr(), n, torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "exl3b200_token_logprobs")
-    return TokenLogprobs(both[0], both[1], top_lp, top_ids)
+        _lib.launch("exl3b200_token_logprobs", index, logits.data_ptr(), logits.stride(0), rows, vocab,
+                    _OUT_DTYPES[logits.dtype], tokens.data_ptr(), top, got[0].data_ptr(), got[1].data_ptr(),
+                    got[2].data_ptr() if top else None, got[3].data_ptr() if top else None, scratch.data_ptr(), n)
+    return got

@@ -15,7 +15,6 @@ whole batch; these operators serve batches whose sequences differ, around the EX
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
@@ -26,20 +25,24 @@ _IN = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.flo
 _CACHE = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float8_e4m3fn: _lib.DTYPE_E4M3}
 
 
-def _on(dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+_E4M3 = torch.float8_e4m3fn
+
+
+def _on(index: int, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             raise RuntimeError("paged tensors must share a CUDA device")
 
 
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor],
-           v_scale: Optional[torch.Tensor]) -> _lib.PagedCache:
+           v_scale: Optional[torch.Tensor]) -> tuple:
+    """The fields of ``exl3b200_paged_cache``."""
     if not k_cache.is_cuda:
         raise RuntimeError("EXL3 B200 ops require CUDA tensors (there is no CPU path)")
-    if k_cache.dtype not in _CACHE or k_cache.dim() != 4 or k_cache.size(3) not in (64, 128):
+    dtype, shape, strides = k_cache.dtype, k_cache.shape, k_cache.stride()
+    if dtype not in _CACHE or len(shape) != 4 or shape[3] not in (64, 128):
         raise RuntimeError("caches must be fp16, bf16 or float8_e4m3fn [pages, page_size, kv_heads, 64 or 128]")
-    shape, strides = k_cache.shape, k_cache.stride()
-    if v_cache.dtype != k_cache.dtype or v_cache.shape != shape or v_cache.stride() != strides:
+    if v_cache.dtype != dtype or v_cache.shape != shape or v_cache.stride() != strides:
         raise RuntimeError("k and v caches must have the same type, shape and strides")
     if strides[3] != 1:
         raise RuntimeError("caches must have unit stride in their last dimension")
@@ -47,23 +50,24 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch
     if not (pages and page_size and kv_heads):
         raise RuntimeError("caches must not be empty")
     st = [s if n > 1 else 0 for s, n in zip(strides, shape)]
-    if any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+    if (pages > 1 and not st[0]) or (page_size > 1 and not st[1]) or (kv_heads > 1 and not st[2]):
         raise RuntimeError("caches must not be expanded views")
-    for s in (k_scale, v_scale):
+    scales = [0, 0]
+    for i, s in enumerate((k_scale, v_scale)):
         if s is not None:
-            if k_cache.dtype != torch.float8_e4m3fn:
+            if dtype != _E4M3:
                 raise RuntimeError("k_scale and v_scale belong to float8_e4m3fn caches")
             if s.dtype != torch.float32 or s.numel() != kv_heads or not s.is_contiguous():
                 raise RuntimeError("k_scale and v_scale must be contiguous fp32 [kv_heads]")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), _CACHE[k_cache.dtype], pages, page_size, kv_heads,
-                           dim, st[0], st[1], st[2], k_scale.data_ptr() if k_scale is not None else None,
-                           v_scale.data_ptr() if v_scale is not None else None)
+            scales[i] = s.data_ptr()
+    return (k_cache.data_ptr(), v_cache.data_ptr(), _CACHE[dtype], pages, page_size, kv_heads, dim, st[0], st[1], st[2],
+            scales[0], scales[1])
 
 
 def _aligned(t: torch.Tensor) -> bool:
-    step = 16 // t.element_size()
-    s = t.stride()
-    return s[2] == 1 and s[0] % step == 0 and s[1] % step == 0 and t.data_ptr() % 16 == 0
+    s0, s1, s2 = t.stride()
+    step = 4 if t.dtype == torch.float32 else 8  # elements of 16 bytes
+    return s2 == 1 and (s0 | s1) % step == 0 and t.data_ptr() % 16 == 0
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -86,27 +90,28 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     in ``ops.device_status``.  The slots of one call must differ.  ``q_out`` (default: new,
     in the cache's type, bf16 for an e4m3 cache) may be ``q``."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
-    dev = k_cache.device
-    _on(dev, q, k, v, positions, slots, inv_freq, q_out, k_scale, v_scale)
-    if q.dtype not in _IN or k.dtype != q.dtype or v.dtype != q.dtype:
+    index = k_cache.get_device()
+    _on(index, v_cache, q, k, v, positions, slots, inv_freq, q_out, k_scale, v_scale)
+    src, cache = q.dtype, k_cache.dtype
+    if src not in _IN or k.dtype != src or v.dtype != src:
         raise RuntimeError("q, k and v must be of one type: fp16, bf16 or fp32")
-    if q.dim() != 3 or q.size(2) != c.head_dim:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != c[6]:
         raise RuntimeError("q must be [tokens, q_heads, head_dim]")
-    tokens, heads, dim = q.shape
-    if k.shape != (tokens, c.kv_heads, dim) or v.shape != k.shape:
+    tokens, heads, dim = shape
+    if k.shape != (tokens, c[5], dim) or v.shape != (tokens, c[5], dim):
         raise RuntimeError("k and v must be [tokens, kv_heads, head_dim]")
-    for t in (positions, slots):
-        if t.dtype != torch.int64 or t.shape != (tokens,):
-            raise RuntimeError("positions and slots must be int64 [tokens]")
+    if (positions.dtype != torch.int64 or slots.dtype != torch.int64 or positions.shape != (tokens,)
+            or slots.shape != (tokens,)):
+        raise RuntimeError("positions and slots must be int64 [tokens]")
     rotary = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float32 or rotary > dim or rotary % 16:
         raise RuntimeError("inv_freq must be fp32 with half of the rotated dims, a multiple of 8 up to head_dim / 2")
-    q_type = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
     if q_out is None:
-        q_out = torch.empty((tokens, heads, dim), dtype=q_type, device=dev)
-    elif q_out.shape != q.shape or q_out.dtype not in (torch.float16, torch.bfloat16):
+        q_out = torch.empty(shape, dtype=torch.bfloat16 if cache == _E4M3 else cache, device=q.device)
+    elif q_out.shape != shape or q_out.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("q_out must be fp16 or bf16, shaped like q")
-    elif k_cache.dtype != torch.float8_e4m3fn and q_out.dtype != q_type:
+    elif cache != _E4M3 and q_out.dtype != cache:
         raise RuntimeError("q_out must have the cache's type")
     elif not _aligned(q_out):
         raise RuntimeError("q_out's heads must begin on 16-byte boundaries with unit stride")
@@ -114,13 +119,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
         return q_out
     q, k, v = _rows(q), _rows(k), _rows(v)
     positions, slots, inv_freq = positions.contiguous(), slots.contiguous(), inv_freq.contiguous()
-    args = _lib.RopeAppendArgs(c, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), positions.data_ptr(),
-                               slots.data_ptr(), inv_freq.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-                               k.stride(1), v.stride(0), v.stride(1), q_out.stride(0), q_out.stride(1), tokens, heads,
-                               rotary, int(bool(interleaved)), _IN[q.dtype], _IN[q_out.dtype])
-    with torch.cuda.device(dev):
-        rc = _lib.lib().exl3b200_rope_append(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "exl3b200_rope_append")
+    args = _lib.pack_rope_append(*c, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), positions.data_ptr(),
+                                 slots.data_ptr(), inv_freq.data_ptr(), *q.stride()[:2], *k.stride()[:2],
+                                 *v.stride()[:2], *q_out.stride()[:2], tokens, heads, rotary, int(bool(interleaved)),
+                                 _IN[src], _IN[q_out.dtype])
+    _lib.launch("exl3b200_rope_append", index, args)
     return q_out
 
 
@@ -142,43 +145,40 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     Rows that see nothing (an empty sequence) are zeros, their ``lse`` is -inf.  Returns
     ``out`` (q's type), with ``return_lse`` also fp32 ``lse [rows, q_heads]``."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
-    dev = k_cache.device
-    _on(dev, q, block_table, seq_lens, k_scale, v_scale, out)
-    if q.dtype not in (torch.float16, torch.bfloat16) or q.dim() != 3 or q.size(2) != c.head_dim:
+    index = k_cache.get_device()
+    _on(index, v_cache, q, block_table, seq_lens, k_scale, v_scale, out)
+    dtype, shape = q.dtype, q.shape
+    if dtype not in (torch.float16, torch.bfloat16) or len(shape) != 3 or shape[2] != c[6]:
         raise RuntimeError("q must be fp16 or bf16 [rows, q_heads, head_dim]")
-    if k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
+    if k_cache.dtype not in (dtype, _E4M3):
         raise RuntimeError("q must have the caches' type (or the caches be float8_e4m3fn)")
-    rows, heads, dim = q.shape
-    R = int(rows_per_seq)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.size(1) < 1:
+    rows, heads, dim = shape
+    kv_heads, R, window, softcap = c[5], int(rows_per_seq), int(window), float(softcap)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise RuntimeError("block_table must be int32 [sequences, max_pages] with unit column stride")
     seqs, max_pages = block_table.shape
     if seq_lens.dtype != torch.int32 or seq_lens.shape != (seqs,) or not seq_lens.is_contiguous():
         raise RuntimeError("seq_lens must be contiguous int32 [sequences]")
-    if R < 1 or rows != seqs * R:
-        raise RuntimeError("q must have rows_per_seq rows for each sequence")
-    if heads < 1 or heads % c.kv_heads or R * (heads // c.kv_heads) > _lib.PAGED_MAX_ROWS:
+    if R < 1 or rows != seqs * R or max_pages < 1:
+        raise RuntimeError("q must have rows_per_seq rows for each sequence, block_table a column")
+    if heads < 1 or heads % kv_heads or R * (heads // kv_heads) > _lib.PAGED_MAX_ROWS:
         raise RuntimeError(f"q_heads must be a multiple of kv_heads, rows_per_seq * group at most {_lib.PAGED_MAX_ROWS}")
-    if int(window) < 0 or not 0.0 <= float(softcap) < float("inf"):
+    if window < 0 or not 0.0 <= softcap < float("inf"):
         raise RuntimeError("window and softcap must not be negative")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or not _aligned(out):
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype != dtype or not _aligned(out):
         raise RuntimeError("out must be shaped like q, of its type, heads on 16-byte boundaries with unit stride")
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if rows:
         q = _rows(q)
-        L = _lib.lib()
-        n = L.exl3b200_paged_attention_scratch_size(R, heads, c.kv_heads, dim)
-        args = _lib.PagedAttentionArgs(c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
-                                       block_table.data_ptr(), seq_lens.data_ptr(), q.stride(0), q.stride(1),
-                                       out.stride(0), out.stride(1), block_table.stride(0) if seqs > 1 else max_pages,
-                                       seqs, R, heads, max_pages, min(int(window), 2 ** 31 - 1), _IN[q.dtype],
-                                       dim ** -0.5 if scale is None else float(scale), float(softcap))
+        n = _lib.lib().exl3b200_paged_attention_scratch_size(R, heads, kv_heads, dim)
         # the scratch is the call's own (a captured graph keeps its own, too)
-        scratch = torch.empty(n, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = L.exl3b200_paged_attention(ctypes.byref(args), scratch.data_ptr(), n,
-                                            torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "exl3b200_paged_attention")
+        scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
+        args = _lib.pack_paged_attention(*c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                                         block_table.data_ptr(), seq_lens.data_ptr(), *q.stride()[:2],
+                                         *out.stride()[:2], block_table.stride(0) if seqs > 1 else max_pages, seqs, R,
+                                         heads, max_pages, min(window, 2 ** 31 - 1), _IN[dtype],
+                                         dim ** -0.5 if scale is None else float(scale), softcap)
+        _lib.launch("exl3b200_paged_attention", index, args, scratch.data_ptr(), n)
     return (out, lse) if return_lse else out

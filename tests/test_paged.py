@@ -98,3 +98,18 @@ def test_cpu_tensors_are_refused():
         paged.rope_append(x, x, x, kc, kc, one, one, torch.zeros(64))
     with pytest.raises(RuntimeError, match="no CPU path"):
         paged.attention(x, kc, kc, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+
+
+def test_packed_arguments_have_the_structs_layout():
+    def fields(st):
+        out = []
+        for name, t in st._fields_:
+            v = getattr(st, name)
+            out += fields(v) if isinstance(v, ctypes.Structure) else [v or 0]
+        return out
+
+    for cls, pack in ((_lib.RopeAppendArgs, _lib.pack_rope_append), (_lib.PagedAttentionArgs, _lib.pack_paged_attention)):
+        raw = bytes((37 * i + 1) % 120 for i in range(ctypes.sizeof(cls)))
+        st = cls.from_buffer_copy(raw)
+        again = cls.from_buffer_copy(pack(*fields(st)))
+        assert len(pack(*fields(st))) == ctypes.sizeof(cls) and fields(again) == fields(st)
