@@ -345,6 +345,12 @@ __device__ __forceinline__ float rcp(float x)
     return r;
 }
 
+// Weights are 2^(score - reference + kRef), a score at most 2^kSlack above the reference.
+// fp16 weights reach 2^14 so that small ones keep their bits: what is lost of a weight is
+// under 2^-31 of the largest.
+constexpr float kSlack = 8.f;
+template <typename MT> __host__ __device__ constexpr float weight_ref() { return std::is_same<MT, __half>::value ? 6.f : 0.f; }
+
 template <int D, bool F8> struct AttnShape {
     static constexpr int kRowBytes = D * (F8 ? 1 : 2);
     static constexpr int kChunks = kRowBytes / 16;           // 16-byte pieces of a row
@@ -396,7 +402,10 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 {
     using S = AttnShape<D, F8>;
     using MT = typename std::conditional<F8, __half, QT>::type;      // the MMAs' type
-    constexpr int kRef = std::is_same<MT, __half>::value ? 14 : 0;   // fp16 weights: up to 2^14, so that small ones keep their bits
+    constexpr float kRef = weight_ref<MT>();
+    // An e4m3 cache with bf16 queries takes the weights as one fp16 each, off by 2^-11 at most
+    // beside the 2^-8 of the output's rounding; the others as hi + lo pairs.
+    constexpr bool kLo = !(F8 && std::is_same<QT, __nv_bfloat16>::value);
     constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
     constexpr bool kQShared = NT > 2;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -663,24 +672,20 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 for (int i = 0; i < 4; ++i) s[0][i] += s2[i];
             // scale, cap, mask; the tiles' maxima
             const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 && (a.window <= 0 || ps >= w.len - a.window);
-            const float capl = a.softcap * kLog2e, icap = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
-            float mx[NT][2];
+            const float capl = a.softcap * kLog2e, icap = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
+            float lg[NT][2], mx[NT][2];  // the factor to base 2 of a row's scores (positive), and the lane's largest score
+            bool grew = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float r0 = ks, r1 = ks;
+                lg[nt][0] = lg[nt][1] = ks * kLog2e;
                 if constexpr (kRowScale) {
                     const float2 t = *reinterpret_cast<const float2*>(&sh_rs[8 * nt + 2 * c]);
-                    r0 = t.x, r1 = t.y;
+                    lg[nt][0] = t.x * kLog2e, lg[nt][1] = t.y * kLog2e;
                 }
                 if (a.softcap > 0.f) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + exp(2 x / cap)))
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = ex2(s[nt][i] * ((i & 1) ? r1 : r0) * icap);
-                        s[nt][i] = fmaf(-2.f * capl, rcp(1.f + e), capl);
-                    }
-                } else {
-                    const float l0 = r0 * kLog2e, l1 = r1 * kLog2e;
-                    s[nt][0] *= l0, s[nt][1] *= l1, s[nt][2] *= l0, s[nt][3] *= l1;
+                    for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[nt][i] * lg[nt][i & 1] * icap)), capl);
+                    lg[nt][0] = lg[nt][1] = 1.f;
                 }
                 if (!open) {
 #pragma unroll
@@ -690,15 +695,15 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                         if (pos >= end || (a.window > 0 && pos < end - a.window)) s[nt][i] = -INFINITY;
                     }
                 }
-                mx[nt][0] = fmaxf(s[nt][0], s[nt][2]);
-                mx[nt][1] = fmaxf(s[nt][1], s[nt][3]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mx[nt][i] = fmaxf(s[nt][i], s[nt][2 + i]) * lg[nt][i];
+                    grew |= mx[nt][i] > rm[nt][i] + kSlack;
+                }
             }
-            bool grew = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) grew |= mx[nt][i] > rm[nt][i];
-            if (__any_sync(~0u, grew)) {  // some row's maximum rises
+            // The weights' reference is a maximum seen, raised only when a score exceeds it by
+            // 2^kSlack: the outputs so far are rescaled in few of the steps.
+            if (__any_sync(~0u, grew)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float al[2];
@@ -720,20 +725,24 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     }
                 }
             }
-            // weights, as B fragments (rows x positions) in hi + lo parts
-            uint32_t hi[NT][2], lo[NT][2];
+            // weights, as B fragments (rows x positions)
+            uint32_t hi[NT][2], lo[NT][kLo ? 2 : 1];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float f0 = rm[nt][0] == -INFINITY ? 0.f : rm[nt][0] - (float) kRef;
-                const float f1 = rm[nt][1] == -INFINITY ? 0.f : rm[nt][1] - (float) kRef;
+                const float f0 = rm[nt][0] == -INFINITY ? 0.f : kRef - rm[nt][0];
+                const float f1 = rm[nt][1] == -INFINITY ? 0.f : kRef - rm[nt][1];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const float x = ex2(s[nt][2 * hf] - f0), y = ex2(s[nt][2 * hf + 1] - f1);
+                    const float x = ex2(fmaf(s[nt][2 * hf], lg[nt][0], f0)), y = ex2(fmaf(s[nt][2 * hf + 1], lg[nt][1], f1));
                     rl[nt][0] += x;
                     rl[nt][1] += y;
-                    split2(x, y, hi[nt][hf], lo[nt][hf], MT());
+                    if constexpr (kLo) {
+                        split2(x, y, hi[nt][hf], lo[nt][hf], MT());
+                        lo[nt][hf] = pg_transpose(lo[nt][hf]);
+                    } else {
+                        hi[nt][hf] = pack2(x, y, MT());
+                    }
                     hi[nt][hf] = pg_transpose(hi[nt][hf]);
-                    lo[nt][hf] = pg_transpose(lo[nt][hf]);
                 }
             }
             if constexpr (F8) {
@@ -750,7 +759,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[nt][0], hi[nt][1]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[nt][0], lo[nt][1]);
+                        for (int nt = 0; kLo && nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[nt][0], lo[nt][kLo]);
                     }
                 }
             } else {
@@ -761,7 +770,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[nt][0], hi[nt][1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[nt][0], lo[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[nt][0], lo[nt][kLo]);
                 }
             }
         }
@@ -831,7 +840,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                         QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + d;
                         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv, QT()), pack2(y.z * inv, y.w * inv, QT()));
                         if (a.lse && d == 0)
-                            a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
+                            a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - kRef + log2f(L)) * kLn2;
                     } else {
                         *reinterpret_cast<float4*>(a.part_o + (part * a.mrows + m) * D + d) = y;
                         if (d == 0) a.part_ml[part * a.mrows + m] = make_float2(M, L);
@@ -861,7 +870,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 template <int D, typename QT, bool F8>
 __global__ __launch_bounds__(128) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
 {
-    constexpr int kRef = (F8 || std::is_same<QT, __half>::value) ? 14 : 0;
+    constexpr float kRef = weight_ref<typename std::conditional<F8, __half, QT>::type>();
     griddep_launch();
     griddep_wait();
     const int4 d = a.desc[blockIdx.x];
@@ -910,7 +919,7 @@ __global__ __launch_bounds__(128) void exl3_paged_join_kernel(const __grid_const
 #pragma unroll
     for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2(y[e] * inv, y[e + 1] * inv, QT());
     if (a.lse && lane == 0)
-        a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - (float) kRef + log2f(L)) * kLn2;
+        a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - kRef + log2f(L)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -1083,7 +1092,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     if (need == 0) return kErrBadShape;
     if (p->dtype != kF16 && p->dtype != kBf16) return kErrBadArgument;
     if (c.dtype != kE4m3 && c.dtype != p->dtype) return kErrBadArgument;
-    if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap) || !std::isfinite(p->scale)) return kErrBadArgument;
+    if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap) || !(p->scale > 0.f) || !std::isfinite(p->scale)) return kErrBadArgument;
     if (scratch_bytes < need) return kErrWorkspace;
     if (misaligned(scratch, 256) || misaligned(p->q, 16) || misaligned(p->out, 16)) return kErrUnaligned;
     if (p->q_stride % 8 || p->q_head_stride % 8 || p->out_stride % 8 || p->out_head_stride % 8) return kErrUnaligned;

@@ -165,6 +165,9 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         raise RuntimeError(f"q_heads must be a multiple of kv_heads, rows_per_seq * group at most {_lib.PAGED_MAX_ROWS}")
     if window < 0 or not 0.0 <= softcap < float("inf"):
         raise RuntimeError("window and softcap must not be negative")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise RuntimeError("scale must be positive")
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     elif out.shape != shape or out.dtype != dtype or not _aligned(out):
@@ -179,6 +182,6 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
                                          block_table.data_ptr(), seq_lens.data_ptr(), *q.stride()[:2],
                                          *out.stride()[:2], block_table.stride(0) if seqs > 1 else max_pages, seqs, R,
                                          heads, max_pages, min(window, 2 ** 31 - 1), _IN[dtype],
-                                         dim ** -0.5 if scale is None else float(scale), softcap)
+                                         scale, softcap)
         _lib.launch("exl3b200_paged_attention", index, args, scratch.data_ptr(), n)
     return (out, lse) if return_lse else out
