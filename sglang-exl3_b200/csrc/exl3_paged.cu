@@ -529,9 +529,6 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     int mbase = 0, mcount = 0, item_u = u0, slot = 0;
     bool fresh = true;
     for (int u = u0; u < u1; ++u) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();
-        fill(slot == 0 ? kStages - 1 : slot - 1);
         if (fresh) {  // a new item: its rows of q
             fresh = false;
             item_u = u;
@@ -592,31 +589,36 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     }
                 }
             } else {
-                // a warp a row: lane l holds dims of k slots in the order of the fragments
-                for (int m = warp; m < 8 * NT; m += kAttnWarps) {
-                    const QT* qr = q_row(m);
-                    constexpr int kPer = D / 32;  // dims of a lane, contiguous
-                    uint32_t t[kPer / 2];
+                // a warp a row, all its rows read at once: lane l holds dims D / 32 l ..
+                constexpr int kPer = D / 64, kMine = 8 * NT / kAttnWarps;  // registers of a lane and row, rows of a warp
+                uint32_t t[kMine][kPer];
 #pragma unroll
-                    for (int i = 0; i < kPer / 2; ++i) t[i] = *reinterpret_cast<const uint32_t*>(qr + kPer * lane + 2 * i);
+                for (int k = 0; k < kMine; ++k) {
+                    const QT* qr = q_row(warp + k * kAttnWarps) + 2 * kPer * lane;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) t[k][i] = *reinterpret_cast<const uint32_t*>(qr + 2 * i);
+                }
+#pragma unroll
+                for (int k = 0; k < kMine; ++k) {
+                    const int m = warp + k * kAttnWarps;
                     if constexpr (kRowScale) {
                         float amax = 0.f;
 #pragma unroll
-                        for (int i = 0; i < kPer / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo16(t[i])), fabsf(hi16(t[i]))));
+                        for (int i = 0; i < kPer; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo16(t[k][i])), fabsf(hi16(t[k][i]))));
 #pragma unroll
                         for (int i = 16; i; i >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, i));
                         float down;
                         const float up = power(amax, &down);
                         if (lane == 0) sh_rs[m] = ks * up;
 #pragma unroll
-                        for (int i = 0; i < kPer / 2; ++i) t[i] = pack2(lo16(t[i]) * down, hi16(t[i]) * down, __half());
+                        for (int i = 0; i < kPer; ++i) t[k][i] = pack2(lo16(t[k][i]) * down, hi16(t[k][i]) * down, __half());
                     }
 #pragma unroll
-                    for (int i = 0; i < kPer / 2; ++i) {
-                        const int d = kPer * lane + 2 * i;
+                    for (int i = 0; i < kPer; ++i) {
+                        const int d = 2 * (kPer * lane + i);
                         // e4m3: dims 4c, 4c + 1 of a 16 go to slots 2c, 2c + 1, dims 4c + 2, 4c + 3 to 8 + 2c, 9 + 2c
                         const int at = F8 ? (d & ~15) + ((d & 2) ? 8 : 0) + ((d & 12) >> 1) : d;
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(qsh + m * S::kQPitch + 2 * at), "r"(t[i]) : "memory");
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(qsh + m * S::kQPitch + 2 * at), "r"(t[k][i]) : "memory");
                     }
                 }
             }
@@ -630,6 +632,9 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             }
         }
 
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        fill(slot == 0 ? kStages - 1 : slot - 1);
         const int p0 = (w.c0 + w.c) * S::kUnit + warp * S::kPos;
         const unsigned kb = ring + slot * S::kSlot, vb = kb + S::kPos * S::kRowBytes;
 #pragma unroll 1
@@ -865,45 +870,65 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 }
 
 // Joins the pieces of the items that the CTAs' runs split: block (x, y) takes the item that
-// begins in the run of CTA x and its rows 4y .. 4y + 3, a warp each, in the order of the
-// pieces (so that a result does not depend on timing).
+// begins in the run of CTA x and its rows 8y .. 8y + 7, a warp each, in the order of the
+// pieces (so that a result does not depend on timing).  A chain of loads: the first pieces
+// are read along with the descriptor that says how many there are.
+constexpr int kJoinWarps = 8;
 template <int D, typename QT, bool F8>
-__global__ __launch_bounds__(128) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
+__global__ __launch_bounds__(32 * kJoinWarps) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
 {
     constexpr float kRef = weight_ref<typename std::conditional<F8, __half, QT>::type>();
+    constexpr int V = D / 32, kFirst = 4;
     griddep_launch();
+    const int lane = threadIdx.x & 31;
+    const int m = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+    if (m >= a.mrows) return;
+    const int most = (int) (gridDim.x - 1 - blockIdx.x);  // pieces after the first, at most
+    auto piece = [&](int p) { return (p == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + p)) * a.mrows + m; };
+    auto load = [&](int p, float (&t)[V]) {
+        const float* src = a.part_o + piece(p) * D + lane * V;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(t) = *reinterpret_cast<const float2*>(src);
+    };
     griddep_wait();
     const int4 d = a.desc[blockIdx.x];
-    if (d.z == 0) return;
-    const int lane = threadIdx.x & 31;
-    const int m = blockIdx.y * 4 + (threadIdx.x >> 5);
+    float2 ml = a.part_ml[piece(min(lane, most))];
+    float first[kFirst][V];
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) load(min(i, most), first[i]);
     const int kvh = d.y / a.mblocks, mbase = (d.y - kvh * a.mblocks) * a.mrows;
-    if (m >= min(a.mrows, a.mtotal - mbase)) return;
-    auto piece = [&](int p) { return (p == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + p)) * a.mrows + m; };
-    constexpr int V = D / 32;
-    float M = -INFINITY;
-    for (int p = lane; p < d.z; p += 32) M = fmaxf(M, a.part_ml[piece(p)].x);
+    if (d.z == 0 || m >= a.mtotal - mbase) return;
+    float M = lane < d.z ? ml.x : -INFINITY;
+    for (int p = lane + 32; p < d.z; p += 32) M = fmaxf(M, a.part_ml[piece(p)].x);
 #pragma unroll
     for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
     float L = 0.f, y[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) y[i] = 0.f;
     for (int p0 = 0; p0 < d.z; p0 += 32) {
-        float k = 0.f, l = 0.f;
+        if (p0 > 0 && p0 + lane < d.z) ml = a.part_ml[piece(p0 + lane)];
+        float k = 0.f;
         if (p0 + lane < d.z) {
-            const float2 ml = a.part_ml[piece(p0 + lane)];
-            l = ml.y;
-            k = ml.x == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(ml.x - M);
+            k = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - M);
+            L += k * ml.y;
         }
-        L += k * l;
         const int n = min(32, d.z - p0);
+        int i0 = 0;
+        if (p0 == 0) {
+#pragma unroll
+            for (int i = 0; i < kFirst; ++i) {
+                const float ki = __shfl_sync(~0u, k, i);
+                if (i < n)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[e] += ki * first[i][e];
+            }
+            i0 = kFirst;
+        }
 #pragma unroll 8
-        for (int i = 0; i < n; ++i) {
+        for (int i = i0; i < n; ++i) {
             const float ki = __shfl_sync(~0u, k, i);
-            const float* src = a.part_o + piece(p0 + i) * D + lane * V;
             float t[V];
-            if constexpr (V == 4) *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(src);
-            else *reinterpret_cast<float2*>(t) = *reinterpret_cast<const float2*>(src);
+            load(p0 + i, t);
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] += ki * t[e];
         }
@@ -993,7 +1018,8 @@ static int attn_launch(const AttnArgs& a, int ctas, cudaStream_t st)
     }
     const int rc = paged_launch(kern, dim3((unsigned) ctas), 32 * kAttnWarps, smem, st, a);
     if (rc != kOk) return rc;
-    return paged_launch(exl3_paged_join_kernel<D, QT, F8>, dim3((unsigned) ctas, (unsigned) ((a.mrows + 3) / 4)), 128, 0, st, a);
+    return paged_launch(exl3_paged_join_kernel<D, QT, F8>, dim3((unsigned) ctas, (unsigned) ((a.mrows + kJoinWarps - 1) / kJoinWarps)),
+                        32 * kJoinWarps, 0, st, a);
 }
 
 template <int D, typename QT, bool F8>
