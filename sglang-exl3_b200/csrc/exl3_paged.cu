@@ -298,13 +298,11 @@ __device__ __forceinline__ void pg_cp16(unsigned s, const void* g, int bytes)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(g), "r"(bytes) : "memory");
 }
-// the two e4m3 values of a 16-bit half as an fp16 pair (exact)
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int hi)
+// four e4m3 values as two fp16 pairs (exact)
+__device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi)
 {
-    const unsigned short h = (unsigned short) (hi ? w >> 16 : w);
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
-    return r;
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // weights as 16-bit hi + lo pairs: together about twice the type's significant bits, so
 // that rounding the weights costs nothing beside the rounding of the output
@@ -349,6 +347,7 @@ __device__ __forceinline__ float rcp(float x)
 // fp16 weights reach 2^14 so that small ones keep their bits: what is lost of a weight is
 // under 2^-31 of the largest.
 constexpr float kSlack = 8.f;
+constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing (finite: no case of its own in the loop)
 template <typename MT> __host__ __device__ constexpr float weight_ref() { return std::is_same<MT, __half>::value ? 6.f : 0.f; }
 
 template <int D, bool F8> struct AttnShape {
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     constexpr bool kLo = !(F8 && std::is_same<QT, __nv_bfloat16>::value);
     constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
     constexpr bool kQShared = NT > 2;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
     __shared__ float sh_rs[kRowScale ? 8 * NT : 1];
     griddep_launch();
@@ -522,10 +521,11 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fill(i);
 
+    const int k_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_row = F8 ? k_row : (lane & 7) + ((lane >> 4) << 3);
     uint32_t qf[kQShared ? 1 : D / 16][NT][2];  // B fragments of q
     float o[D / 16][NT][4];                     // O^T: dims g, g + 8 of a 16-dim tile x rows 2c, 2c + 1
     float rm[NT][2], rl[NT][2];                 // rows 2c, 2c + 1 of a tile: running maximum (base 2), this lane's sum
-    float ks = 0.f;
+    float ks = 0.f;                             // the scores' scale, to base 2
     int mbase = 0, mcount = 0, item_u = u0, slot = 0;
     bool fresh = true;
     for (int u = u0; u < u1; ++u) {
@@ -535,7 +535,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             const int kvh = w.h / a.mblocks, mb = w.h - kvh * a.mblocks;
             mbase = mb * a.mrows;
             mcount = min(a.mrows, a.mtotal - mbase);
-            ks = (F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale;
+            ks = ((F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale) * kLog2e;
             // row m of the item (rows past its last repeat it and are not written)
             auto q_row = [&](int m) {
                 const int mm = mbase + min(m, mcount - 1), j = mm / a.group;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             if constexpr (kQShared || kRowScale) __syncthreads();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                rm[nt][0] = rm[nt][1] = -INFINITY;
+                rm[nt][0] = rm[nt][1] = kNone;
                 rl[nt][0] = rl[nt][1] = 0.f;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
@@ -641,6 +641,10 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
         for (int sb = 0; sb < S::kPos / 16; ++sb) {
             const int ps = p0 + 16 * sb;
             if (ps >= w.len || ps + 16 <= w.lo) continue;  // warp-uniform
+            // this lane's row and first piece of a tile of K and of V; other pieces differ in the
+            // pieces' bits alone (a row begins on a boundary of its pieces)
+            const unsigned ka = kb + S::at(16 * sb + k_row, lane >> 4);
+            const unsigned va = vb + S::at(16 * sb + v_row, F8 ? lane >> 4 : (lane >> 3) & 1);
             // scores: positions g, g + 8 x rows 2c, 2c + 1 of every tile
             float s[NT][4];
 #pragma unroll
@@ -651,13 +655,14 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 uint32_t k0[4], k1[4];
                 if constexpr (F8) {
                     uint32_t r[4];
-                    pg_ldsm4(r, kb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), kk + (lane >> 4)));
-                    k0[0] = e4m3x2_f16x2(r[0], 0), k0[1] = e4m3x2_f16x2(r[1], 0), k0[2] = e4m3x2_f16x2(r[0], 1), k0[3] = e4m3x2_f16x2(r[1], 1);
-                    k1[0] = e4m3x2_f16x2(r[2], 0), k1[1] = e4m3x2_f16x2(r[3], 0), k1[2] = e4m3x2_f16x2(r[2], 1), k1[3] = e4m3x2_f16x2(r[3], 1);
+                    pg_ldsm4(r, ka ^ (16 * kk));
+                    e4m3x4_f16x2(r[0], k0[0], k0[2]);
+                    e4m3x4_f16x2(r[1], k0[1], k0[3]);
+                    e4m3x4_f16x2(r[2], k1[0], k1[2]);
+                    e4m3x4_f16x2(r[3], k1[1], k1[3]);
                 } else {
-                    const int row = (lane & 7) + (((lane >> 3) & 1) << 3);
-                    pg_ldsm4(k0, kb + S::at(row, 2 * kk + (lane >> 4)));
-                    pg_ldsm4(k1, kb + S::at(row, 2 * kk + 2 + (lane >> 4)));
+                    pg_ldsm4(k0, ka ^ (32 * kk));
+                    pg_ldsm4(k1, ka ^ (32 * kk + 32));
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -675,51 +680,57 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             if (NT == 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[0][i] += s2[i];
-            // scale, cap, mask; the tiles' maxima
+            // cap and mask
             const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 && (a.window <= 0 || ps >= w.len - a.window);
-            const float capl = a.softcap * kLog2e, icap = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
-            float lg[NT][2], mx[NT][2];  // the factor to base 2 of a row's scores (positive), and the lane's largest score
-            bool grew = false;
+            // the factors that take rows 2c, 2c + 1 of a tile to base 2 (positive)
+            auto factor = [&](int nt) {
+                float2 t = make_float2(ks, ks);
+                if constexpr (kRowScale) t = *reinterpret_cast<const float2*>(&sh_rs[8 * nt + 2 * c]);
+                return t;
+            };
+            const bool capped = a.softcap > 0.f;
+            if (capped) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + exp(2 x / cap)))
+                const float capl = a.softcap * kLog2e, icap = 2.f / a.softcap;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                lg[nt][0] = lg[nt][1] = ks * kLog2e;
-                if constexpr (kRowScale) {
-                    const float2 t = *reinterpret_cast<const float2*>(&sh_rs[8 * nt + 2 * c]);
-                    lg[nt][0] = t.x * kLog2e, lg[nt][1] = t.y * kLog2e;
-                }
-                if (a.softcap > 0.f) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + exp(2 x / cap)))
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float2 t = factor(nt);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[nt][i] * lg[nt][i & 1] * icap)), capl);
-                    lg[nt][0] = lg[nt][1] = 1.f;
+                    for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[nt][i] * ((i & 1) ? t.y : t.x) * icap)), capl);
                 }
-                if (!open) {
+            }
+            if (!open) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int end = w.len - a.rows + 1 + (mbase + min(8 * nt + 2 * c + (i & 1), mcount - 1)) / a.group;
                         const int pos = ps + g + 8 * (i >> 1);
                         if (pos >= end || (a.window > 0 && pos < end - a.window)) s[nt][i] = -INFINITY;
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    mx[nt][i] = fmaxf(s[nt][i], s[nt][2 + i]) * lg[nt][i];
-                    grew |= mx[nt][i] > rm[nt][i] + kSlack;
-                }
             }
             // The weights' reference is a maximum seen, raised only when a score exceeds it by
             // 2^kSlack: the outputs so far are rescaled in few of the steps.
-            if (__any_sync(~0u, grew)) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float2 t = factor(nt);
+                if (capped) t = make_float2(1.f, 1.f);
+                top = fmaxf(top, fmaxf(fmaf(fmaxf(s[nt][0], s[nt][2]), t.x, -rm[nt][0]), fmaf(fmaxf(s[nt][1], s[nt][3]), t.y, -rm[nt][1])));
+            }
+            if (__any_sync(~0u, top > kSlack)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
+                    float2 t = factor(nt);
+                    if (capped) t = make_float2(1.f, 1.f);
                     float al[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float x = mx[nt][i];
+                        float x = fmaxf(s[nt][i], s[nt][2 + i]) * (i ? t.y : t.x);
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
                         x = fmaxf(x, rm[nt][i]);
-                        al[i] = rm[nt][i] == -INFINITY ? 0.f : ex2(rm[nt][i] - x);
+                        al[i] = ex2(rm[nt][i] - x);
                         rm[nt][i] = x;
                         rl[nt][i] *= al[i];
                     }
@@ -734,11 +745,12 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             uint32_t hi[NT][2], lo[NT][kLo ? 2 : 1];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float f0 = rm[nt][0] == -INFINITY ? 0.f : kRef - rm[nt][0];
-                const float f1 = rm[nt][1] == -INFINITY ? 0.f : kRef - rm[nt][1];
+                float2 t = factor(nt);
+                if (capped) t = make_float2(1.f, 1.f);
+                const float f0 = kRef - rm[nt][0], f1 = kRef - rm[nt][1];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const float x = ex2(fmaf(s[nt][2 * hf], lg[nt][0], f0)), y = ex2(fmaf(s[nt][2 * hf + 1], lg[nt][1], f1));
+                    const float x = ex2(fmaf(s[nt][2 * hf], t.x, f0)), y = ex2(fmaf(s[nt][2 * hf + 1], t.y, f1));
                     rl[nt][0] += x;
                     rl[nt][1] += y;
                     if constexpr (kLo) {
@@ -755,12 +767,12 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                 for (int j = 0; j < D / 16; j += 2) {
                     uint32_t r[4];
-                    pg_ldsm4t(r, vb + S::at(16 * sb + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
+                    pg_ldsm4t(r, va ^ (16 * j));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t ev = __byte_perm(r[2 * i], r[2 * i + 1], 0x6420);
-                        const uint32_t od = __byte_perm(r[2 * i], r[2 * i + 1], 0x7531);
-                        const uint32_t v[4] = {e4m3x2_f16x2(ev, 0), e4m3x2_f16x2(od, 0), e4m3x2_f16x2(ev, 1), e4m3x2_f16x2(od, 1)};
+                        uint32_t v[4];
+                        e4m3x4_f16x2(__byte_perm(r[2 * i], r[2 * i + 1], 0x6420), v[0], v[2]);
+                        e4m3x4_f16x2(__byte_perm(r[2 * i], r[2 * i + 1], 0x7531), v[1], v[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[nt][0], hi[nt][1]);
 #pragma unroll
@@ -771,7 +783,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
                     uint32_t v[4];
-                    pg_ldsm4t(v, vb + S::at((lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)));
+                    pg_ldsm4t(v, va ^ (32 * j));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[nt][0], hi[nt][1]);
 #pragma unroll
@@ -790,7 +802,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 4);
                     rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 8);
                     rl[nt][i] += __shfl_xor_sync(~0u, rl[nt][i], 16);
-                    if (g == 0) sh_m[warp][8 * nt + 2 * c + i] = rm[nt][i], sh_l[warp][8 * nt + 2 * c + i] = rl[nt][i];
+                    if (g == 0) sh_m[warp][8 * nt + 2 * c + i] = rm[nt][i] > kNone ? rm[nt][i] : -INFINITY, sh_l[warp][8 * nt + 2 * c + i] = rl[nt][i];
                 }
             const bool whole = w.c == w.n - 1 && u - item_u == w.n - 1;
             const bool starts = w.c == u - item_u;  // the piece holds the item's first unit
