@@ -353,11 +353,11 @@ template <typename MT> __host__ __device__ constexpr float weight_ref() { return
 template <int D, bool F8> struct AttnShape {
     static constexpr int kRowBytes = D * (F8 ? 1 : 2);
     static constexpr int kChunks = kRowBytes / 16;           // 16-byte pieces of a row
-    static constexpr int kPos = F8 ? 32 : 16;                // positions of a warp's stage
+    static constexpr int kPos = kRowBytes == 256 ? 16 : 32;  // positions of a warp's stage
     static constexpr int kUnit = kAttnWarps * kPos;          // positions of a CTA's stage
     static constexpr int kSlot = 2 * kPos * kRowBytes;       // bytes of K and V
     static constexpr int kQPitch = 2 * D + 16;               // bytes of a row of q in shared memory
-    static_assert(kSlot == 16 * D * 4, "a stage holds 16 rows of a warp's partial output at the end of an item");
+    static_assert(kSlot >= 16 * D * 4 && (kSlot & (kSlot - 1)) == 0, "a stage holds 16 rows of a warp's partial output at the end of an item");
     // 16-byte piece c of row r, so that eight rows of a piece column lie in distinct banks
     static __device__ __forceinline__ int at(int r, int c)
     {
@@ -407,6 +407,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     constexpr bool kLo = !(F8 && std::is_same<QT, __nv_bfloat16>::value);
     constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
     constexpr bool kQShared = NT > 2;
+    constexpr int kBlocks = S::kPos == 32 && NT <= 2 ? 2 : 1;  // 16-position blocks of a step
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
     __shared__ float sh_rs[kRowScale ? 8 * NT : 1];
@@ -638,20 +639,25 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
         const int p0 = (w.c0 + w.c) * S::kUnit + warp * S::kPos;
         const unsigned kb = ring + slot * S::kSlot, vb = kb + S::kPos * S::kRowBytes;
 #pragma unroll 1
-        for (int sb = 0; sb < S::kPos / 16; ++sb) {
+        for (int sb = 0; sb < S::kPos / 16; sb += kBlocks) {
             const int ps = p0 + 16 * sb;
-            if (ps >= w.len || ps + 16 <= w.lo) continue;  // warp-uniform
+            if (ps >= w.len || ps + 16 * kBlocks <= w.lo) continue;  // warp-uniform
             // this lane's row and first piece of a tile of K and of V; other pieces differ in the
             // pieces' bits alone (a row begins on a boundary of its pieces)
-            const unsigned ka = kb + S::at(16 * sb + k_row, lane >> 4);
-            const unsigned va = vb + S::at(16 * sb + v_row, F8 ? lane >> 4 : (lane >> 3) & 1);
+            const unsigned ka0 = kb + S::at(16 * sb + k_row, lane >> 4);
+            const unsigned va0 = vb + S::at(16 * sb + v_row, F8 ? lane >> 4 : (lane >> 3) & 1);
             // scores: positions g, g + 8 x rows 2c, 2c + 1 of every tile
-            float s[NT][4];
+            float s[kBlocks][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-            float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile: a second chain of accumulations
+            for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int kk = 0; kk < D / 16; kk += 2) {
+                for (int nt = 0; nt < NT; ++nt) s[b][nt][0] = s[b][nt][1] = s[b][nt][2] = s[b][nt][3] = 0.f;
+            float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile of one block: a second chain of accumulations
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk += 2)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const unsigned ka = ka0 + b * 16 * S::kRowBytes;
                 uint32_t k0[4], k1[4];
                 if constexpr (F8) {
                     uint32_t r[4];
@@ -669,19 +675,19 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     if constexpr (kQShared) {
                         uint32_t r[4];
                         pg_ldsm4(r, qsh + (8 * nt + (lane & 7)) * S::kQPitch + 32 * kk + 16 * (lane >> 3));
-                        mma16816<MT>(s[nt], k0, r[0], r[1]);
-                        mma16816<MT>(s[nt], k1, r[2], r[3]);
+                        mma16816<MT>(s[b][nt], k0, r[0], r[1]);
+                        mma16816<MT>(s[b][nt], k1, r[2], r[3]);
                     } else {
-                        mma16816<MT>(s[nt], k0, qf[kk][nt][0], qf[kk][nt][1]);
-                        mma16816<MT>(NT == 1 ? s2 : s[nt], k1, qf[kk + 1][nt][0], qf[kk + 1][nt][1]);
+                        mma16816<MT>(s[b][nt], k0, qf[kk][nt][0], qf[kk][nt][1]);
+                        mma16816<MT>(NT == 1 && kBlocks == 1 ? s2 : s[b][nt], k1, qf[kk + 1][nt][0], qf[kk + 1][nt][1]);
                     }
                 }
             }
-            if (NT == 1)
+            if (NT == 1 && kBlocks == 1)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[0][i] += s2[i];
+                for (int i = 0; i < 4; ++i) s[0][0][i] += s2[i];
             // cap and mask
-            const bool open = ps >= w.lo && ps + 16 <= w.len - a.rows + 1 && (a.window <= 0 || ps >= w.len - a.window);
+            const bool open = ps >= w.lo && ps + 16 * kBlocks <= w.len - a.rows + 1 && (a.window <= 0 || ps >= w.len - a.window);
             // the factors that take rows 2c, 2c + 1 of a tile to base 2 (positive)
             auto factor = [&](int nt) {
                 float2 t = make_float2(ks, ks);
@@ -695,7 +701,10 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 for (int nt = 0; nt < NT; ++nt) {
                     const float2 t = factor(nt);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[nt][i] * ((i & 1) ? t.y : t.x) * icap)), capl);
+                    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[b][nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[b][nt][i] * ((i & 1) ? t.y : t.x) * icap)), capl);
                 }
             }
             if (!open) {
@@ -704,18 +713,26 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int end = w.len - a.rows + 1 + (mbase + min(8 * nt + 2 * c + (i & 1), mcount - 1)) / a.group;
-                        const int pos = ps + g + 8 * (i >> 1);
-                        if (pos >= end || (a.window > 0 && pos < end - a.window)) s[nt][i] = -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b) {
+                            const int pos = ps + 16 * b + g + 8 * (i >> 1);
+                            if (pos >= end || (a.window > 0 && pos < end - a.window)) s[b][nt][i] = -INFINITY;
+                        }
                     }
             }
             // The weights' reference is a maximum seen, raised only when a score exceeds it by
             // 2^kSlack: the outputs so far are rescaled in few of the steps.
+            auto largest = [&](int nt, int i) {  // of the lane's scores in row 2c + i
+                float x = fmaxf(s[0][nt][i], s[0][nt][2 + i]);
+                if constexpr (kBlocks == 2) x = fmaxf(x, fmaxf(s[1][nt][i], s[1][nt][2 + i]));
+                return x;
+            };
             float top = -INFINITY;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float2 t = factor(nt);
                 if (capped) t = make_float2(1.f, 1.f);
-                top = fmaxf(top, fmaxf(fmaf(fmaxf(s[nt][0], s[nt][2]), t.x, -rm[nt][0]), fmaf(fmaxf(s[nt][1], s[nt][3]), t.y, -rm[nt][1])));
+                top = fmaxf(top, fmaxf(fmaf(largest(nt, 0), t.x, -rm[nt][0]), fmaf(largest(nt, 1), t.y, -rm[nt][1])));
             }
             if (__any_sync(~0u, top > kSlack)) {
 #pragma unroll
@@ -725,7 +742,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     float al[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float x = fmaxf(s[nt][i], s[nt][2 + i]) * (i ? t.y : t.x);
+                        float x = largest(nt, i) * (i ? t.y : t.x);
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
@@ -742,52 +759,57 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 }
             }
             // weights, as B fragments (rows x positions)
-            uint32_t hi[NT][2], lo[NT][kLo ? 2 : 1];
+            uint32_t hi[kBlocks][NT][2], lo[kBlocks][NT][kLo ? 2 : 1];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float2 t = factor(nt);
                 if (capped) t = make_float2(1.f, 1.f);
                 const float f0 = kRef - rm[nt][0], f1 = kRef - rm[nt][1];
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float x = ex2(fmaf(s[nt][2 * hf], t.x, f0)), y = ex2(fmaf(s[nt][2 * hf + 1], t.y, f1));
+                for (int bh = 0; bh < 2 * kBlocks; ++bh) {
+                    const int b = bh >> 1, hf = bh & 1;
+                    const float x = ex2(fmaf(s[b][nt][2 * hf], t.x, f0)), y = ex2(fmaf(s[b][nt][2 * hf + 1], t.y, f1));
                     rl[nt][0] += x;
                     rl[nt][1] += y;
                     if constexpr (kLo) {
-                        split2(x, y, hi[nt][hf], lo[nt][hf], MT());
-                        lo[nt][hf] = pg_transpose(lo[nt][hf]);
+                        split2(x, y, hi[b][nt][hf], lo[b][nt][hf], MT());
+                        lo[b][nt][hf] = pg_transpose(lo[b][nt][hf]);
                     } else {
-                        hi[nt][hf] = pack2(x, y, MT());
+                        hi[b][nt][hf] = pack2(x, y, MT());
                     }
-                    hi[nt][hf] = pg_transpose(hi[nt][hf]);
+                    hi[b][nt][hf] = pg_transpose(hi[b][nt][hf]);
                 }
             }
             if constexpr (F8) {
                 // 16 dims of V: rows g of the A fragment are dims 2g, rows g + 8 dims 2g + 1
 #pragma unroll
-                for (int j = 0; j < D / 16; j += 2) {
+                for (int j = 0; j < D / 16; j += 2)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
                     uint32_t r[4];
-                    pg_ldsm4t(r, va ^ (16 * j));
+                    pg_ldsm4t(r, (va0 + b * 16 * S::kRowBytes) ^ (16 * j));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t v[4];
                         e4m3x4_f16x2(__byte_perm(r[2 * i], r[2 * i + 1], 0x6420), v[0], v[2]);
                         e4m3x4_f16x2(__byte_perm(r[2 * i], r[2 * i + 1], 0x7531), v[1], v[3]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[nt][0], hi[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[b][nt][0], hi[b][nt][1]);
 #pragma unroll
-                        for (int nt = 0; kLo && nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[nt][0], lo[nt][kLo]);
+                        for (int nt = 0; kLo && nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[b][nt][0], lo[b][nt][kLo]);
                     }
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) {
+                for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
                     uint32_t v[4];
-                    pg_ldsm4t(v, va ^ (32 * j));
+                    pg_ldsm4t(v, (va0 + b * 16 * S::kRowBytes) ^ (32 * j));
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[nt][0], hi[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[b][nt][0], hi[b][nt][1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[nt][0], lo[nt][kLo]);
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[b][nt][0], lo[b][nt][kLo]);
                 }
             }
         }
