@@ -410,7 +410,10 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     constexpr int kBlocks = S::kPos == 32 && NT <= 2 ? 2 : 1;  // 16-position blocks of a step
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
-    __shared__ float sh_rs[kRowScale ? 8 * NT : 1];
+    __shared__ __align__(8) float sh_rs[kRowScale ? 8 * NT : 1];
+    __shared__ long long sh_q[8 * NT];                // the item's rows: offset in q,
+    __shared__ int sh_out[8 * NT];                    // row * q_heads + head,
+    __shared__ __align__(8) int sh_end[8 * NT];       // and the positions below which are seen
     griddep_launch();
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -537,12 +540,15 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             mbase = mb * a.mrows;
             mcount = min(a.mrows, a.mtotal - mbase);
             ks = ((F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale) * kLog2e;
-            // row m of the item (rows past its last repeat it and are not written)
-            auto q_row = [&](int m) {
-                const int mm = mbase + min(m, mcount - 1), j = mm / a.group;
-                return reinterpret_cast<const QT*>(a.q) + ((long long) w.s * a.rows + j) * a.q_row +
-                       (long long) (kvh * a.group + mm - j * a.group) * a.q_head;
-            };
+            if (tid < 8 * NT) {  // (rows past the item's last repeat it and are not written)
+                const int mm = mbase + min(tid, mcount - 1), j = mm / a.group;
+                const int row = w.s * a.rows + j, head = kvh * a.group + mm - j * a.group;
+                sh_q[tid] = row * a.q_row + head * a.q_head;
+                sh_out[tid] = row * (a.kv_heads * a.group) + head;
+                sh_end[tid] = w.len - a.rows + 1 + j;
+            }
+            __syncthreads();
+            auto q_row = [&](int m) { return reinterpret_cast<const QT*>(a.q) + sh_q[m]; };
             // An e4m3 cache meets q in fp16, to which e4m3 converts exactly; a bf16 row is taken
             // into fp16's range by a power of two that the scores' scale takes back.  Four bytes
             // of a cache row come to a lane: dims 4c .. 4c + 3 of each 16 are its k slots.
@@ -590,36 +596,38 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     }
                 }
             } else {
-                // a warp a row, all its rows read at once: lane l holds dims D / 32 l ..
-                constexpr int kPer = D / 64, kMine = 8 * NT / kAttnWarps;  // registers of a lane and row, rows of a warp
+                // eight lanes a row, D / 8 dims each; all rows read at once
+                constexpr int kPer = D / 16;                                  // pairs of a lane and row
+                constexpr int kMine = (8 * NT + 4 * kAttnWarps - 1) / (4 * kAttnWarps);
                 uint32_t t[kMine][kPer];
+                const int r0 = 4 * warp + (lane >> 3), l8 = lane & 7;
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
-                    const QT* qr = q_row(warp + k * kAttnWarps) + 2 * kPer * lane;
+                    const QT* qr = q_row(min(r0 + 4 * kAttnWarps * k, 8 * NT - 1)) + 2 * kPer * l8;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i) t[k][i] = *reinterpret_cast<const uint32_t*>(qr + 2 * i);
+                    for (int i = 0; i < kPer; i += 4) *reinterpret_cast<uint4*>(&t[k][i]) = *reinterpret_cast<const uint4*>(qr + 2 * i);
                 }
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
-                    const int m = warp + k * kAttnWarps;
+                    const int m = r0 + 4 * kAttnWarps * k;
+                    float down = 1.f, up = 1.f;
                     if constexpr (kRowScale) {
                         float amax = 0.f;
 #pragma unroll
                         for (int i = 0; i < kPer; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo16(t[k][i])), fabsf(hi16(t[k][i]))));
 #pragma unroll
-                        for (int i = 16; i; i >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, i));
-                        float down;
-                        const float up = power(amax, &down);
-                        if (lane == 0) sh_rs[m] = ks * up;
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) t[k][i] = pack2(lo16(t[k][i]) * down, hi16(t[k][i]) * down, __half());
+                        for (int i = 4; i; i >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, i));
+                        up = power(amax, &down);
                     }
+                    if (m >= 8 * NT) continue;
+                    if (kRowScale && l8 == 0) sh_rs[m] = ks * up;
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) {
-                        const int d = 2 * (kPer * lane + i);
+                        const uint32_t x = kRowScale ? pack2(lo16(t[k][i]) * down, hi16(t[k][i]) * down, __half()) : t[k][i];
+                        const int d = 2 * (kPer * l8 + i);
                         // e4m3: dims 4c, 4c + 1 of a 16 go to slots 2c, 2c + 1, dims 4c + 2, 4c + 3 to 8 + 2c, 9 + 2c
                         const int at = F8 ? (d & ~15) + ((d & 2) ? 8 : 0) + ((d & 12) >> 1) : d;
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(qsh + m * S::kQPitch + 2 * at), "r"(t[k][i]) : "memory");
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(qsh + m * S::kQPitch + 2 * at), "r"(x) : "memory");
                     }
                 }
             }
@@ -712,7 +720,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int end = w.len - a.rows + 1 + (mbase + min(8 * nt + 2 * c + (i & 1), mcount - 1)) / a.group;
+                        const int end = sh_end[8 * nt + 2 * c + (i & 1)];
 #pragma unroll
                         for (int b = 0; b < kBlocks; ++b) {
                             const int pos = ps + 16 * b + g + 8 * (i >> 1);
@@ -872,14 +880,11 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                         }
                     }
                     if (whole) {
-                        const int mm = mbase + m, j = mm / a.group;
-                        const long long row = (long long) w.s * a.rows + j;
-                        const int head = kvh * a.group + mm - j * a.group;
+                        const int at = sh_out[m], row = at / (a.kv_heads * a.group), head = at - row * (a.kv_heads * a.group);
                         const float inv = L == 0.f ? 0.f : vs / L;
                         QT* dst = reinterpret_cast<QT*>(a.out) + row * a.out_row + head * a.out_head + d;
                         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv, QT()), pack2(y.z * inv, y.w * inv, QT()));
-                        if (a.lse && d == 0)
-                            a.lse[row * (a.kv_heads * a.group) + head] = L == 0.f ? -INFINITY : (M - kRef + log2f(L)) * kLn2;
+                        if (a.lse && d == 0) a.lse[at] = L == 0.f ? -INFINITY : (M - kRef + log2f(L)) * kLn2;
                     } else {
                         *reinterpret_cast<float4*>(a.part_o + (part * a.mrows + m) * D + d) = y;
                         if (d == 0) a.part_ml[part * a.mrows + m] = make_float2(M, L);
@@ -1161,7 +1166,9 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     const AttnSplit sp = attn_split(p->rows_per_seq, p->q_heads / c.kv_heads, c.head_dim);
     // positions are 32-bit, and so is the number of units of a launch
     const long long capacity = std::min((long long) p->max_pages * c.page_size, (long long) INT_MAX - 256);
-    if (((capacity + 63) / 64 + 1) * p->seqs * c.kv_heads * sp.mblocks > INT_MAX) return kErrBadShape;
+    if (((capacity + 63) / 64 + 1) * p->seqs * c.kv_heads * sp.mblocks > INT_MAX ||
+        (long long) p->seqs * p->rows_per_seq * p->q_heads > INT_MAX)
+        return kErrBadShape;
     a.q = p->q, a.out = p->out, a.lse = p->lse;
     a.k = reinterpret_cast<const unsigned char*>(c.k), a.v = reinterpret_cast<const unsigned char*>(c.v);
     a.table = p->block_table, a.lens = p->seq_lens, a.table_row = p->table_stride;
