@@ -7,8 +7,9 @@
 //
 // in base 2 throughout (y = x log2(e) - M2).  Rows of 16-bit or fp32 logits are cut into
 // units of 256 vectors of 8 elements; every CTA takes an equal contiguous run of the units
-// of all rows, so that one row fills the machine as well as thousands do, and the pieces of
-// a row that lies in several runs are joined by a second kernel in a fixed order.
+// of all rows (of one row, where there are more CTAs than rows), so that one row fills the
+// machine as well as thousands do, and the pieces of a row that lies in several runs are
+// joined by a second kernel in a fixed order.
 //
 // Alternatives: each thread keeps the maximum of the vectors it saw and the vector that held
 // it, and the second largest vector maximum.  The k-th largest of the threads' maxima is a
@@ -51,7 +52,17 @@ struct LogprobArgs {
     u64* part_keys;       // [2 ctas][top]
     long long row_stride;
     int rows, vocab, top, row_units;
+    int row_ctas;         // CTAs of a row when there are more CTAs than rows, else 0
 };
+
+// The run of units of CTA b: an equal share of all units, or - when there are several CTAs to
+// a row - of one row's, so that no CTA finishes two pieces.
+__host__ __device__ __forceinline__ long long lp_run(const LogprobArgs& a, int b, int ctas)
+{
+    if (a.row_ctas == 0) return b * ((long long) a.rows * a.row_units) / ctas;
+    const int row = b / a.row_ctas;
+    return (long long) row * a.row_units + (long long) (b - row * a.row_ctas) * a.row_units / a.row_ctas;
+}
 
 __device__ __forceinline__ float lp_ex2(float x)
 {
@@ -59,12 +70,59 @@ __device__ __forceinline__ float lp_ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// a lower bound on an exponent that lets a NaN through
+// a lower bound of -200 on an exponent that lets a NaN through
 __device__ __forceinline__ float lp_bound(float y)
 {
     float r;
-    asm("max.NaN.f32 %0, %1, 0fC3480000;" : "=f"(r) : "f"(y));  // -200
+    asm("max.NaN.f32 %0, %1, 0fC3480000;" : "=f"(r) : "f"(y));
     return r;
+}
+// two fp32 operations in one instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 lp_pair(float a, float b)
+{
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void lp_unpair(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 lp_fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 lp_add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// max of packed 16-bit pairs; the NaN form lets a NaN through
+template <typename T> __device__ __forceinline__ uint32_t lp_max2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint32_t lp_low2(uint32_t a)
+{
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xFBFFFBFFu));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xF149F149u));
+    return r;
+}
+__device__ __forceinline__ float lp_low(float x)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fF149F2CA;" : "=f"(r) : "f"(x));  // -1e30
+    return r;
+}
+template <typename T> __device__ __forceinline__ float2 lp_float2(uint32_t w)
+{
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 // order of the values as unsigned integers (0 is below every value; -0 counts as 0)
 __device__ __forceinline__ unsigned lp_order(float x)
@@ -181,8 +239,13 @@ template <typename T> struct LpRow {
     __device__ __forceinline__ int vectors() const { return (end + kLpVec - 1) / kLpVec; }
 };
 
-// a finite logit for which (x - M) is taken instead of x log2 e - M2, whose product might overflow
-__device__ __forceinline__ bool lp_far(float M) { return fabsf(M) > 1e29f && fabsf(M) < INFINITY; }
+// A finite logit for which (x - M) is taken instead of x log2 e - M2: its product might
+// overflow, or it is near the bound to which the main loop lifts -inf (so that y e is 0 and
+// not NaN): -1e30, in fp16 the lowest value.
+template <typename T> __device__ __forceinline__ bool lp_far(float M)
+{
+    return (fabsf(M) > 1e29f && fabsf(M) < INFINITY) || (std::is_same<T, __half>::value && M < -3e4f && M > -INFINITY);
+}
 
 // A row's results from its maximum M, S and T (relative to M2 = M log2 e) and warp 0's
 // descending keys.
@@ -190,7 +253,7 @@ template <typename T>
 __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, float M, float S, float Tt, u64 key, int tid)
 {
     const float M2 = M * kLpLog2e, ls = log2f(S);
-    auto of = [&](float x) { return lp_far(M) || lp_far(x) ? (x - M) - ls * kLpLn2 : (fmaf(x, kLpLog2e, -M2) - ls) * kLpLn2; };
+    auto of = [&](float x) { return lp_far<T>(M) || lp_far<T>(x) ? (x - M) - ls * kLpLn2 : (fmaf(x, kLpLog2e, -M2) - ls) * kLpLn2; };
     if (tid == 0) {
         const long long t = a.tokens[row];
         float lp = -INFINITY;  // an id outside the vocabulary has no probability
@@ -219,9 +282,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
     griddep_launch();
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const long long total = (long long) a.rows * a.row_units;
-    int u = (int) (blockIdx.x * total / gridDim.x);
-    const int u_end = (int) ((blockIdx.x + 1) * total / gridDim.x);
+    int u = (int) lp_run(a, blockIdx.x, gridDim.x);
+    const int u_end = (int) lp_run(a, blockIdx.x + 1, gridDim.x);
     while (u < u_end) {
         const int row = u / a.row_units;
         const int c0 = u - row * a.row_units, c1 = min(a.row_units, c0 + (u_end - u));  // units of the row: the piece
@@ -229,10 +291,10 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
         const LpRow<T> r(a, row);
         const int nv = r.vectors();
         const int v0 = c0 * kLpThreads + tid, v1 = min(nv, c1 * kLpThreads);  // vectors v0, v0 + 256, ... of this thread
-        float best = -INFINITY, second = -INFINITY, ref = -1e30f, s = 0.f, t = 0.f;
+        float best = -INFINITY, second = -INFINITY, ref = -1e30f;
+        f32x2 s2 = lp_pair(0.f, 0.f), t2 = s2;
         int bv = v0;
-        auto take = [&](const float (&f)[8], int v) {
-            const float cm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+        auto top_of = [&](float cm, int v) {  // a vector's maximum
             second = fmaxf(second, fminf(best, cm));
             if (cm > best) {
                 best = cm;
@@ -240,27 +302,59 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
                 const float c2 = cm * kLpLog2e;
                 if (c2 > ref + kLpSlack) {
                     const float d = ref - c2, k = lp_ex2(d);
-                    t = (t + d * s) * k;
-                    s *= k;
+                    float s0, s1, t0, t1;
+                    lp_unpair(s2, s0, s1);
+                    lp_unpair(t2, t0, t1);
+                    t2 = lp_pair((t0 + d * s0) * k, (t1 + d * s1) * k);
+                    s2 = lp_pair(s0 * k, s1 * k);
                     ref = c2;
                 }
             }
+        };
+        auto add = [&](float x0, float x1) {  // finite or NaN
+            const f32x2 y = lp_fma2(lp_pair(x0, x1), lp_pair(kLpLog2e, kLpLog2e), lp_pair(-ref, -ref));
+            float y0, y1;
+            lp_unpair(y, y0, y1);
+            const f32x2 e = lp_pair(lp_ex2(y0), lp_ex2(y1));
+            s2 = lp_add2(s2, e);
+            t2 = lp_fma2(y, e, t2);
+        };
+        auto take = [&](const LpVec<T>& x, int v) {
+            if constexpr (sizeof(T) == 4) {
+                float f[8];
+                x.get(f);
+                top_of(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // (a -inf gives y e = 0 through the bound)
-                const float y = lp_bound(fmaf(f[i], kLpLog2e, -ref));
-                const float e = lp_ex2(y);
-                s += e;
-                t = fmaf(y, e, t);
+                for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
+            } else {
+                const uint4 w = x.w[0];
+                const float2 m = lp_float2<T>(lp_max2<T>(lp_max2<T>(w.x, w.y), lp_max2<T>(w.z, w.w)));
+                top_of(fmaxf(m.x, m.y), v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = lp_float2<T>(lp_low2<T>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w));
+                    add(f.x, f.y);
+                }
+            }
+        };
+        auto take_any = [&](int v) {
+            if (r.inside(v)) {
+                LpVec<T> x;
+                x.load(r.p + (long long) v * kLpVec);
+                take(x, v);
+            } else {
+                float f[8];
+                r.edge(v, f);
+                top_of(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), v);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
             }
         };
         {
             constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
             int v = v0;
             if (v < v1 && !r.inside(v)) {
-                float f[8];
-                r.edge(v, f);
-                take(f, v);
+                take_any(v);
                 v += kLpThreads;
             }
             for (; v + (kAhead - 1) * kLpThreads < v1 && r.inside(v + (kAhead - 1) * kLpThreads); v += kAhead * kLpThreads) {
@@ -268,17 +362,17 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) x[i].load(r.p + (long long) (v + i * kLpThreads) * kLpVec);
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    float f[8];
-                    x[i].get(f);
-                    take(f, v + i * kLpThreads);
-                }
+                for (int i = 0; i < kAhead; ++i) take(x[i], v + i * kLpThreads);
             }
-            for (; v < v1; v += kLpThreads) {
-                float f[8];
-                r.read(v, f);
-                take(f, v);
-            }
+            for (; v < v1; v += kLpThreads) take_any(v);
+        }
+        float s, t;
+        {
+            float s1, t1;
+            lp_unpair(s2, s, s1);
+            lp_unpair(t2, t, t1);
+            s += s1;
+            t += t1;
         }
 
         // M, S, T of the piece
@@ -290,7 +384,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kLpWarps; ++i) M = fmaxf(M, red[i][0]);
-        if (lp_far(M)) {  // logits whose product with log2 e leaves fp32's exact range, as a mask of the type's lowest value
+        if (lp_far<T>(M)) {  // logits whose product with log2 e leaves fp32's exact range, as a mask of the type's lowest value
             s = t = 0.f;
             for (int v = v0; v < v1; v += kLpThreads) {
                 float f[8];
@@ -402,22 +496,27 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
     }
 }
 
-// The row that begins in the run of CTA x of the first kernel and does not end there.
+// The row that begins in the run of CTA b of the first kernel and does not end there
+// (b: this block, or the first CTA of its row).
 template <typename T>
-__global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __grid_constant__ LogprobArgs a)
+__global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __grid_constant__ LogprobArgs a, int ctas)
 {
     __shared__ u64 lists[kLpWarps][32];
     griddep_launch();
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const long long total = (long long) a.rows * a.row_units;
-    const long long u0 = blockIdx.x * total / gridDim.x, u1 = (blockIdx.x + 1) * total / gridDim.x;
-    if (u0 == u1) return;
-    const int row = (int) ((u1 - 1) / a.row_units);  // the run's last row
-    const long long first = (long long) row * a.row_units, last = first + a.row_units - 1;
-    if (first < u0 || last < u1) return;  // began earlier, or ends here
-    const int pieces = (int) (((last + 1) * gridDim.x - 1) / total) - (int) blockIdx.x + 1;
-    auto at = [&](int p) { return p == 0 ? 2 * (int) blockIdx.x + 1 : 2 * ((int) blockIdx.x + p); };
+    const int cta = a.row_ctas ? blockIdx.x * a.row_ctas : blockIdx.x;
+    int row = blockIdx.x, pieces = a.row_ctas;
+    if (!a.row_ctas) {
+        const long long total = (long long) a.rows * a.row_units;
+        const long long u0 = lp_run(a, cta, ctas), u1 = lp_run(a, cta + 1, ctas);
+        if (u0 == u1) return;
+        row = (int) ((u1 - 1) / a.row_units);  // the run's last row
+        const long long first = (long long) row * a.row_units, last = first + a.row_units - 1;
+        if (first < u0 || last < u1) return;  // began earlier, or ends here
+        pieces = (int) (((last + 1) * ctas - 1) / total) - cta + 1;
+    }
+    auto at = [&](int p) { return p == 0 ? 2 * cta + 1 : 2 * (cta + p); };
     float M = -INFINITY, S = 0.f, Tt = 0.f;
     if (warp == 0) {
         for (int p = lane; p < pieces; p += 32) M = fmaxf(M, a.part[at(p)].x);
@@ -425,7 +524,7 @@ __global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __
         for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
         for (int p = lane; p < pieces; p += 32) {
             const float4 q = a.part[at(p)];
-            const float d = lp_far(M) ? (q.x - M) * kLpLog2e : q.x * kLpLog2e - M * kLpLog2e, k = lp_ex2(d);
+            const float d = lp_far<T>(M) ? (q.x - M) * kLpLog2e : q.x * kLpLog2e - M * kLpLog2e, k = lp_ex2(d);
             S += q.y * k;
             Tt += k == 0.f ? 0.f : (q.z + d * q.y) * k;
         }
@@ -449,9 +548,20 @@ __global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __
     if (warp == 0) lp_write<T>(a, row, M, S, Tt, key, tid);
 }
 
-static int lp_ctas(long long rows, int row_units) { return (int) std::min<long long>(kLpCtas, rows * row_units); }
 // (a row that does not begin on a 16-byte boundary reaches over one vector more)
 static int lp_row_units(int vocab) { return (int) (((long long) vocab + kLpVec - 1 + kLpUnit - 1) / kLpUnit); }
+
+struct LpSplit {
+    int ctas, row_ctas;
+};
+static LpSplit lp_split(long long rows, int row_units)
+{
+    if (rows < kLpCtas) {
+        const int p = std::min<int>((int) (kLpCtas / rows), row_units);
+        return {(int) rows * p, p};
+    }
+    return {kLpCtas, 0};
+}
 
 template <typename T> static int lp_launch(const LogprobArgs& a, int ctas, cudaStream_t st)
 {
@@ -465,8 +575,9 @@ template <typename T> static int lp_launch(const LogprobArgs& a, int ctas, cudaS
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, exl3_logprobs_kernel<T>, a) != cudaSuccess) return kErrLaunch;
-    if ((long long) a.rows * a.row_units % ctas == 0 && (long long) a.rows * a.row_units / ctas % a.row_units == 0) return kOk;  // no run cuts a row
-    return cudaLaunchKernelEx(&cfg, exl3_logprobs_join_kernel<T>, a) == cudaSuccess ? kOk : kErrLaunch;
+    if (a.row_ctas == 1 || (a.row_ctas == 0 && a.rows % ctas == 0)) return kOk;  // no run cuts a row
+    if (a.row_ctas) cfg.gridDim = dim3((unsigned) a.rows);
+    return cudaLaunchKernelEx(&cfg, exl3_logprobs_join_kernel<T>, a, ctas) == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace exl3b200
@@ -478,7 +589,7 @@ extern "C" size_t exl3b200_token_logprobs_scratch_size(int rows, int vocab, int 
     if (rows < 1 || vocab < 1 || vocab > (1 << 30) || top < 0 || top > kLpMaxTop || top > vocab) return 0;
     const int units = lp_row_units(vocab);
     if ((long long) rows * units > INT_MAX) return 0;
-    const size_t ctas = (size_t) lp_ctas(rows, units);
+    const size_t ctas = (size_t) lp_split(rows, units).ctas;
     return 2 * ctas * (sizeof(float4) + (size_t) top * sizeof(u64));
 }
 
@@ -497,7 +608,9 @@ extern "C" int exl3b200_token_logprobs(const void* logits, long long row_stride,
     a.logits = logits, a.tokens = tokens, a.logprob = logprob, a.entropy = entropy;
     a.top_logprob = top_logprobs, a.top_ids = top_ids;
     a.row_stride = row_stride, a.rows = rows, a.vocab = vocab, a.top = top, a.row_units = lp_row_units(vocab);
-    const int ctas = lp_ctas(rows, a.row_units);
+    const LpSplit sp = lp_split(rows, a.row_units);
+    const int ctas = sp.ctas;
+    a.row_ctas = sp.row_ctas;
     a.part = reinterpret_cast<float4*>(scratch);
     a.part_keys = reinterpret_cast<u64*>(a.part + 2 * ctas);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
