@@ -294,22 +294,30 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
         float best = -INFINITY, second = -INFINITY, ref = -1e30f;
         f32x2 s2 = lp_pair(0.f, 0.f), t2 = s2;
         int bv = v0;
-        auto top_of = [&](float cm, int v) {  // a vector's maximum
-            second = fmaxf(second, fminf(best, cm));
-            if (cm > best) {
-                best = cm;
-                bv = v;
-                const float c2 = cm * kLpLog2e;
-                if (c2 > ref + kLpSlack) {
-                    const float d = ref - c2, k = lp_ex2(d);
-                    float s0, s1, t0, t1;
-                    lp_unpair(s2, s0, s1);
-                    lp_unpair(t2, t0, t1);
-                    t2 = lp_pair((t0 + d * s0) * k, (t1 + d * s1) * k);
-                    s2 = lp_pair(s0 * k, s1 * k);
-                    ref = c2;
-                }
+        // vectors b .. b + n of the row into L2, one request of one thread
+        auto prefetch = [&](int b, int n) {
+            const int lo = max(b, r.inside(0) ? 0 : 1), hi = min(b + n, min(v1, r.end / kLpVec));
+            if (tid == 0 && hi > lo) {
+                const char* p = reinterpret_cast<const char*>(r.p + (long long) lo * kLpVec);
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((hi - lo) * kLpVec * (int) sizeof(T)) : "memory");
             }
+        };
+        auto raise = [&](float cm) {  // before elements of at most cm are added
+            const float c2 = cm * kLpLog2e;
+            if (c2 > ref + kLpSlack) {
+                const float d = ref - c2, k = lp_ex2(d);
+                float s0, s1, t0, t1;
+                lp_unpair(s2, s0, s1);
+                lp_unpair(t2, t0, t1);
+                t2 = lp_pair((t0 + d * s0) * k, (t1 + d * s1) * k);
+                s2 = lp_pair(s0 * k, s1 * k);
+                ref = c2;
+            }
+        };
+        auto rank = [&](float cm, int v) {  // a vector's maximum among this thread's
+            second = fmaxf(second, fminf(best, cm));
+            bv = cm > best ? v : bv;
+            best = fmaxf(best, cm);
         };
         auto add = [&](float x0, float x1) {  // finite or NaN
             const f32x2 y = lp_fma2(lp_pair(x0, x1), lp_pair(kLpLog2e, kLpLog2e), lp_pair(-ref, -ref));
@@ -319,50 +327,68 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
             s2 = lp_add2(s2, e);
             t2 = lp_fma2(y, e, t2);
         };
-        auto take = [&](const LpVec<T>& x, int v) {
+        auto max8 = [](const float (&f)[8]) {
+            return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+        };
+        auto largest = [&](const LpVec<T>& x) {
             if constexpr (sizeof(T) == 4) {
                 float f[8];
                 x.get(f);
-                top_of(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), v);
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
+                return max8(f);
             } else {
                 const uint4 w = x.w[0];
                 const float2 m = lp_float2<T>(lp_max2<T>(lp_max2<T>(w.x, w.y), lp_max2<T>(w.z, w.w)));
-                top_of(fmaxf(m.x, m.y), v);
+                return fmaxf(m.x, m.y);
+            }
+        };
+        auto add8 = [&](const LpVec<T>& x) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    const uint4 w = x.w[i >> 1];
+                    add(lp_low(__uint_as_float(i & 1 ? w.z : w.x)), lp_low(__uint_as_float(i & 1 ? w.w : w.y)));
+                } else {
+                    const uint4 w = x.w[0];
                     const float2 f = lp_float2<T>(lp_low2<T>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w));
                     add(f.x, f.y);
                 }
             }
         };
         auto take_any = [&](int v) {
-            if (r.inside(v)) {
-                LpVec<T> x;
-                x.load(r.p + (long long) v * kLpVec);
-                take(x, v);
-            } else {
-                float f[8];
-                r.edge(v, f);
-                top_of(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), v);
+            float f[8];
+            r.read(v, f);
+            const float cm = max8(f);
+            raise(cm);
+            rank(cm, v);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
-            }
+            for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
         };
         {
             constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+            constexpr int kFar = 2;
+            prefetch(c0 * kLpThreads, kFar * kAhead * kLpThreads);
             int v = v0;
             if (v < v1 && !r.inside(v)) {
                 take_any(v);
                 v += kLpThreads;
             }
             for (; v + (kAhead - 1) * kLpThreads < v1 && r.inside(v + (kAhead - 1) * kLpThreads); v += kAhead * kLpThreads) {
+                prefetch(v - tid + kFar * kAhead * kLpThreads, kAhead * kLpThreads);
                 LpVec<T> x[kAhead];
+                float cm[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) x[i].load(r.p + (long long) (v + i * kLpThreads) * kLpVec);
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) take(x[i], v + i * kLpThreads);
+                for (int i = 0; i < kAhead; ++i) cm[i] = largest(x[i]);
+                float all = cm[0];
+#pragma unroll
+                for (int i = 1; i < kAhead; ++i) all = fmaxf(all, cm[i]);
+                raise(all);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    rank(cm[i], v + i * kLpThreads);
+                    add8(x[i]);
+                }
             }
             for (; v < v1; v += kLpThreads) take_any(v);
         }
@@ -422,8 +448,18 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
             }
             best_vec[tid] = bv;
             const u64 mine = key;
-            key = lp_merge_warps(lp_sort(key, lane), lists, warp, lane);
-            if (a.top > 1) {
+            if (a.top == 1) {  // the largest of the threads' largest
+#pragma unroll
+                for (int i = 16; i; i >>= 1) {
+                    const u64 o = __shfl_xor_sync(~0u, key, i);
+                    key = o > key ? o : key;
+                }
+                if (lane == 0) lists[0][warp] = key;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kLpWarps; ++i) key = lists[0][i] > key ? lists[0][i] : key;
+            } else {
+                key = lp_merge_warps(lp_sort(key, lane), lists, warp, lane);
                 if (warp == 0 && lane == a.top - 1) sh_bound = key;
                 __syncthreads();
                 u64 bound = sh_bound;
