@@ -10,7 +10,10 @@ bf16.  Two step implementations:
   SwiGLU in the gate/up epilogue - about a dozen kernels per layer;
 * unfused: one grouped launch for q/k/v, one for o, one for gate/up, one for
   down, with RMSNorm, RoPE, KV append, SiLU*mul and attention
-  (``scaled_dot_product_attention``) in plain torch.  Under
+  (``scaled_dot_product_attention``) in plain torch;
+* paged (``paged=True``): the unfused step over a paged cache, every sequence at a
+  position of its own (``exl3_b200.paged``: RoPE and the append to the pages in one
+  kernel, attention over the pages), in bf16 or e4m3.  Under
 tensor parallelism (one process per GPU) q/k/v/gate/up are column shards, o/down
 row shards followed by an NCCL all-reduce, and lm_head is sharded by vocabulary
 with an all-gather of the logits.  A decode step (one token per sequence) is
@@ -31,7 +34,8 @@ import ctypes
 import torch
 import torch.nn.functional as F
 
-from . import _lib, ops
+from . import _lib, ops, paged
+from .logprobs import TokenLogprobs, token_logprobs
 
 
 @dataclass
@@ -72,7 +76,15 @@ def exl3_weight_bytes(cfg: DecoderConfig, world: int = 1) -> int:
 class DecodeModel:
     def __init__(self, cfg: DecoderConfig, batch: int, max_ctx: int, device: torch.device, world: int = 1,
                  rank: int = 0, group=None, seed: int = 3, fused: Optional[bool] = None, peer: bool = True,
-                 fold: bool = True):
+                 fold: bool = True, paged: bool = False, page_size: int = 64,
+                 kv_dtype: torch.dtype = torch.bfloat16, logprobs: Optional[int] = None):
+        """``paged``: a paged cache of ``max_ctx`` positions per sequence, in ``kv_dtype`` (bf16 or
+        float8_e4m3fn); ``self.pos`` is then int64 [batch].  ``logprobs``: report the generated
+        tokens' log-probabilities with that many alternatives (0..32; ``generate`` returns them)."""
+        if paged and fused:
+            raise ValueError("the fused decode layer reads a dense cache")
+        if kv_dtype not in ((torch.bfloat16, torch.float8_e4m3fn) if paged else (torch.bfloat16,)):
+            raise ValueError("kv_dtype must be bf16, or float8_e4m3fn for a paged cache")
         if cfg.heads % world or cfg.kv_heads % world or cfg.inter % (128 * world) or cfg.vocab % world:
             raise ValueError(f"config does not shard over tp={world}")
         self.cfg, self.batch, self.max_ctx, self.device = cfg, batch, max_ctx, device
@@ -98,16 +110,27 @@ class DecodeModel:
         self.v_loc = cfg.vocab // world
         self.lm_head = (torch.randn(self.v_loc, H, generator=gen, device=device) * 0.02).to(torch.bfloat16)
         self.ln_f = torch.ones(H, dtype=torch.bfloat16, device=device)
-        # KV cache: [layer][B, kv_heads_local, max_ctx, head_dim] bf16
-        # zero-filled: the unfused step attends over the whole cache with a mask, and a
-        # masked position holding NaN garbage would still poison the softmax sum
-        self.k_cache = torch.zeros((cfg.layers, batch, self.hkv, max_ctx, hd), dtype=torch.bfloat16, device=device)
+        self.paged, self.page_size, self.n_logprobs = bool(paged), int(page_size), logprobs
+        self.logprobs = None
+        if self.paged:
+            # [layer][pages, page_size, kv_heads_local, head_dim]; a sequence's pages lie apart
+            per_seq = -(-max_ctx // self.page_size)
+            self.k_cache = torch.zeros((cfg.layers, batch * per_seq, self.page_size, self.hkv, hd), dtype=kv_dtype,
+                                       device=device)
+            self.block_table = (torch.arange(per_seq, device=device)[None, :] * batch
+                                + torch.arange(batch, device=device)[:, None]).to(torch.int32)
+            self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        else:
+            # KV cache: [layer][B, kv_heads_local, max_ctx, head_dim] bf16
+            # zero-filled: the unfused step attends over the whole cache with a mask, and a
+            # masked position holding NaN garbage would still poison the softmax sum
+            self.k_cache = torch.zeros((cfg.layers, batch, self.hkv, max_ctx, hd), dtype=torch.bfloat16, device=device)
         self.v_cache = torch.zeros_like(self.k_cache)
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, device=device, dtype=torch.float32) / hd))
         self.inv_freq = inv
         # static step buffers
         self.tokens = torch.zeros(batch, dtype=torch.long, device=device)
-        self.pos = torch.zeros((), dtype=torch.long, device=device)
+        self.pos = torch.zeros(batch if self.paged else (), dtype=torch.long, device=device)
         self.next_tokens = torch.zeros(batch, dtype=torch.long, device=device)
         self.qkv = torch.empty((batch, self.q_out + 2 * self.kv_out), dtype=torch.float16, device=device)
         self.gu = torch.empty((batch, 2 * self.i_loc), dtype=torch.float16, device=device)
@@ -115,7 +138,7 @@ class DecodeModel:
         self.down = torch.empty((batch, H), dtype=torch.float16, device=device)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.ctx = 0
-        self.fused = (batch <= 16) if fused is None else bool(fused)
+        self.fused = (batch <= 16 and not self.paged) if fused is None else bool(fused)
         if self.fused and batch > 16:
             raise ValueError("the fused decode layer takes at most 16 sequences")
         self.h = torch.zeros((batch, H), dtype=torch.float32, device=device)       # residual stream
@@ -136,9 +159,20 @@ class DecodeModel:
             self.layer_descs = [LayerDesc(L["ln1"], L["qkv"], L["o"], L["ln2"], L["gu"][0], L["gu"][1], L["down"])
                                 for L in self.layers]
 
-    def fill_random_kv(self, ctx: int, seed: int = 11):
+    def fill_random_kv(self, ctx, seed: int = 11):
+        """``ctx`` random positions per sequence; paged: a number or one for each sequence."""
         g = torch.Generator(device=self.device)
         g.manual_seed(seed + self.rank)
+        if self.paged:
+            lens = torch.as_tensor(ctx, dtype=torch.long).expand(self.batch)
+            if int(lens.max()) > self.max_ctx:
+                raise ValueError("context beyond max_ctx")
+            for lay in range(self.cfg.layers):
+                for c in (self.k_cache, self.v_cache):
+                    c[lay].copy_(torch.randn(c[lay].shape, generator=g, device=self.device, dtype=torch.bfloat16))
+            self.ctx = lens
+            self.pos.copy_(lens)
+            return
         for lay in range(self.cfg.layers):
             self.k_cache[lay, :, :, :ctx].normal_(generator=g)
             self.v_cache[lay, :, :, :ctx].normal_(generator=g)
@@ -165,6 +199,8 @@ class DecodeModel:
         self.next_tokens (greedy) and appends to the KV cache."""
         if self.fused:
             return self._step_fused()
+        if self.paged:
+            return self._step_paged()
         return self._step_unfused()
 
     def _step_fused(self):
@@ -205,8 +241,44 @@ class DecodeModel:
             logits = torch.cat(parts, dim=-1)
         self.last_logits = logits
         self.next_tokens.copy_(logits.argmax(-1))
+        if self.n_logprobs is not None:
+            self.logprobs = token_logprobs(logits, self.next_tokens, self.n_logprobs)
         self.tokens.copy_(self.next_tokens)
         self.pos.add_(1)
+
+    def _step_paged(self):
+        cfg = self.cfg
+        B, hd, ps = self.batch, cfg.head_dim, self.page_size
+        h = self.embed[self.tokens].float()
+        pos = self.pos
+        # this step's slots, the same for every layer; for a sequence that has filled its pages one
+        # past the pool, which the append records in the device status
+        page = self.block_table.gather(1, (pos // ps).clamp(max=self.block_table.size(1) - 1)[:, None])[:, 0].long()
+        slots = torch.where(pos < self.max_ctx, page * ps + pos % ps, self.k_cache.size(1) * ps)
+        self.seq_lens.copy_((pos + 1).clamp(max=self.max_ctx))
+        for li, L in enumerate(self.layers):
+            x = self._rms(h, L["ln1"])
+            q, k, v = self.qkv[:, :self.q_out], self.qkv[:, self.q_out:self.q_out + self.kv_out], self.qkv[:, self.q_out + self.kv_out:]
+            ops.matmul_multi(x, L["qkv"], cfg.K, cfg.cb, outs=[q, k, v])
+            kc, vc = self.k_cache[li], self.v_cache[li]
+            qr = paged.rope_append(q.view(B, self.hq, hd), k.view(B, self.hkv, hd), v.view(B, self.hkv, hd), kc, vc,
+                                   pos, slots, self.inv_freq)
+            attn = paged.attention(qr, kc, vc, self.block_table, self.seq_lens)
+            ops.matmul(attn.view(B, self.q_out).to(torch.float16), *L["o"], cfg.K, cfg.cb, out=self.o)
+            self._allreduce(self.o)
+            h = self._mlp_unfused(h + self.o.float(), L)
+        self.h.copy_(h)
+        self._finish(h)
+
+    def _mlp_unfused(self, h: torch.Tensor, L) -> torch.Tensor:
+        cfg = self.cfg
+        x = self._rms(h, L["ln2"])
+        g, u = self.gu[:, :self.i_loc], self.gu[:, self.i_loc:]
+        ops.matmul_multi(x, L["gu"], cfg.K, cfg.cb, outs=[g, u])
+        act = (F.silu(g.float()) * u.float()).to(torch.float16)
+        ops.matmul(act, *L["down"], cfg.K, cfg.cb, out=self.down)
+        self._allreduce(self.down)
+        return h + self.down.float()
 
     def _step_unfused(self):
         cfg = self.cfg
@@ -227,14 +299,7 @@ class DecodeModel:
                                                   enable_gqa=True)
             ops.matmul(attn.reshape(B, self.q_out).to(torch.float16), *L["o"], cfg.K, cfg.cb, out=self.o)
             self._allreduce(self.o)
-            h = h + self.o.float()
-            x = self._rms(h, L["ln2"])
-            g, u = self.gu[:, :self.i_loc], self.gu[:, self.i_loc:]
-            ops.matmul_multi(x, L["gu"], cfg.K, cfg.cb, outs=[g, u])
-            act = (F.silu(g.float()) * u.float()).to(torch.float16)
-            ops.matmul(act, *L["down"], cfg.K, cfg.cb, out=self.down)
-            self._allreduce(self.down)
-            h = h + self.down.float()
+            h = self._mlp_unfused(h + self.o.float(), L)
         self.h.copy_(h)
         self._finish(h)
 
@@ -242,19 +307,19 @@ class DecodeModel:
         """Warm up on a side stream and capture one decode step in a CUDA graph."""
         s = stream or torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
-        pos0 = int(self.pos.item())
+        pos0 = self.pos.clone()
         tok0 = self.tokens.clone()
         with torch.cuda.stream(s):
             for _ in range(2):
                 self.step()
-            self.pos.fill_(pos0)
+            self.pos.copy_(pos0)
             self.tokens.copy_(tok0)
             torch.cuda.synchronize(self.device)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, stream=s):
                 self.step()
         torch.cuda.current_stream(self.device).wait_stream(s)
-        self.pos.fill_(pos0)
+        self.pos.copy_(pos0)
         self.tokens.copy_(tok0)
         self.graph = g
         self.stream = s
@@ -281,9 +346,10 @@ class DecodeModel:
             self._host_bufs = buf
         return buf
 
-    def generate(self, prompt_tokens: torch.Tensor, n: int) -> torch.Tensor:
+    def generate(self, prompt_tokens: torch.Tensor, n: int):
         """Public API: greedy-decode n tokens after ``prompt_tokens`` (host [B] last
-        prompt tokens); returns the host [B, n] tokens.  Each step copies its input
+        prompt tokens); returns the host [B, n] tokens - with ``logprobs=k`` at construction
+        also their ``TokenLogprobs`` on the host (``[B, n]`` and ``[B, n, k]``).  Each step copies its input
         tokens from pinned host memory (the previous step's output as the host received
         it) and its output tokens back, then waits for them, as a serving loop does."""
         if self.graph is None:
@@ -292,6 +358,10 @@ class DecodeModel:
         status = self._status_host()
         host_in.copy_(prompt_tokens.to(torch.long))
         L = _lib.lib()
+        lps = None
+        if self.n_logprobs is not None:
+            lps = [None if t is None else torch.empty((self.batch, n) + t.shape[1:], dtype=t.dtype)
+                   for t in self.logprobs]
         with torch.cuda.stream(self.stream):
             for i in range(n):
                 if i > 0:
@@ -305,7 +375,11 @@ class DecodeModel:
                 self.stream.synchronize()
                 if int(status[0]) != 0:
                     raise RuntimeError(f"decode step {i}: device status {_lib.status_string(int(status[0]))}")
-        return host_out[:, :n].clone()
+                for src, dst in zip(self.logprobs, lps) if lps else ():
+                    if dst is not None:
+                        dst[:, i].copy_(src)
+        tokens = host_out[:, :n].clone()
+        return tokens if lps is None else (tokens, TokenLogprobs(*lps))
 
     def _status_host(self) -> torch.Tensor:
         buf = getattr(self, "_status_buf", None)

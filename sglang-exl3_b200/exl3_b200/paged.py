@@ -108,7 +108,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     if inv_freq.dtype != torch.float32 or rotary > dim or rotary % 16:
         raise RuntimeError("inv_freq must be fp32 with half of the rotated dims, a multiple of 8 up to head_dim / 2")
     if q_out is None:
-        q_out = torch.empty(shape, dtype=torch.bfloat16 if cache == _E4M3 else cache, device=q.device)
+        q_out = q.new_empty(shape, dtype=torch.bfloat16 if cache == _E4M3 else cache)
     elif q_out.shape != shape or q_out.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("q_out must be fp16 or bf16, shaped like q")
     elif cache != _E4M3 and q_out.dtype != cache:
@@ -169,15 +169,15 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     if not 0.0 < scale < float("inf"):
         raise RuntimeError("scale must be positive")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != dtype or not _aligned(out):
         raise RuntimeError("out must be shaped like q, of its type, heads on 16-byte boundaries with unit stride")
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if rows:
         q = _rows(q)
         n = _lib.lib().exl3b200_paged_attention_scratch_size(R, heads, kv_heads, dim)
         # the scratch is the call's own (a captured graph keeps its own, too)
-        scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(n, dtype=torch.uint8)
         args = _lib.pack_paged_attention(*c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
                                          block_table.data_ptr(), seq_lens.data_ptr(), *q.stride()[:2],
                                          *out.stride()[:2], block_table.stride(0) if seqs > 1 else max_pages, seqs, R,

@@ -45,6 +45,7 @@ from . import moe as _moe
 from . import ops
 from .ep import PeerExpertParallelMoE
 from .harness import _random_linear
+from .logprobs import TokenLogprobs, token_logprobs
 
 
 @dataclass
@@ -268,6 +269,17 @@ class VerifyModel:
             with torch.cuda.graph(self.graph, stream=s):
                 self.logits = self.step()
         torch.cuda.current_stream(self.device).wait_stream(s)
+
+    def draft_logprobs(self, top: int = 0) -> TokenLogprobs:
+        """The verify step's verdict on the draft: for every row but a sequence's last, the
+        log-probability that the model gives the next drafted token (``self.tokens[:, j + 1]``),
+        its entropy there and the ``top`` tokens it would rather have; the last row has no drafted
+        token (-inf).  Shaped like the rows, ``[batch * rows_per_seq]``, from the step's logits."""
+        if self.logits is None:
+            raise RuntimeError("run a verify step first")
+        want = torch.full_like(self.tokens, -1)
+        want[:, :-1] = self.tokens[:, 1:]
+        return token_logprobs(self.logits, want.view(-1), top)
 
     def replay(self, n: int = 1) -> None:
         with torch.cuda.stream(self.stream):
