@@ -650,16 +650,12 @@ EXL3B200_API int exl3b200_paged_attention(const exl3b200_paged_attention_args* a
  * logits [rows][vocab] F16, BF16 or F32, row stride in elements, any element-aligned base;
  * -inf marks excluded tokens (a row of nothing else, or one with a NaN or +inf, gives NaN).
  * Sums in fp32.  tokens, top_ids: device int64; the other outputs fp32.  top 0..32, at most
- * vocab; with 0 top_logprobs and top_ids may be NULL.  scratch:
- * exl3b200_token_logprobs_scratch_size bytes (0: bad sizes), 16-byte aligned, no
- * initialisation, per concurrent call.  No counterpart in the reference, whose callers take
- * SGLang's sampler.
+ * vocab; with 0 top_logprobs and top_ids may be NULL.  No workspace.  No counterpart in the
+ * reference, whose callers take SGLang's sampler.
  */
-EXL3B200_API size_t exl3b200_token_logprobs_scratch_size(int rows, int vocab, int top);
 EXL3B200_API int exl3b200_token_logprobs(const void* logits, long long row_stride, int rows, int vocab, int dtype,
                                          const long long* tokens, int top, float* logprob, float* entropy,
-                                         float* top_logprobs, long long* top_ids, void* scratch,
-                                         size_t scratch_bytes, void* stream);
+                                         float* top_logprobs, long long* top_ids, void* stream);
 
 /*
  * Checkpoint reader: copies count byte ranges of the open file fd (offsets[i],

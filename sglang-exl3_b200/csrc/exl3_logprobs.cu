@@ -5,11 +5,10 @@
 //   H   = lse - sum_i p_i x_i            = log S - T / S   with y_i = x_i - M,
 //                                          S = sum exp(y_i), T = sum y_i exp(y_i)
 //
-// in base 2 throughout (y = x log2(e) - M2).  Rows of 16-bit or fp32 logits are cut into
-// units of 256 vectors of 8 elements; every CTA takes an equal contiguous run of the units
-// of all rows (of one row, where there are more CTAs than rows), so that one row fills the
-// machine as well as thousands do, and the pieces of a row that lies in several runs are
-// joined by a second kernel in a fixed order.
+// in base 2 throughout (y = x log2(e) - M2).  A row of 16-bit or fp32 logits is cut into
+// units of 256 vectors of 8 elements and is one CTA's, or - when rows are few - a cluster's
+// of up to 8 CTAs, whose first joins the pieces through distributed shared memory in a fixed
+// order.
 //
 // Alternatives: each thread keeps the maximum of the vectors it saw and the vector that held
 // it, and the second largest vector maximum.  The k-th largest of the threads' maxima is a
@@ -20,17 +19,24 @@
 #include <algorithm>
 #include <climits>
 
+#include <cooperative_groups.h>
+
 #include "exl3_common.cuh"
 #include "exl3_capi_internal.h"
 #include "exl3_grouped_dev.cuh"
 
 namespace exl3b200 {
 
+namespace cg = cooperative_groups;
+
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVec = 8;                       // elements of a thread's vector
 constexpr int kLpUnit = kLpThreads * kLpVec;    // elements of a unit
-constexpr int kLpCtas = 4 * 148;
+constexpr int kLpCluster = 8;                   // most CTAs of a row
+// CTAs of a launch with clusters: 4 fit on an SM, but clusters do not pack a GPC's slots fully
+// (80 rows as clusters of 7, 95 % of the slots, took two waves: 27.5 us instead of 18.0 as 6)
+constexpr int kLpClusterCtas = 480;
 constexpr int kLpMaxTop = EXL3B200_LOGPROBS_MAX_TOP;
 constexpr int kLpBuffer = 1024;                 // candidates kept before they are cut back to the best 32
 constexpr float kLpLog2e = 1.4426950408889634f;
@@ -48,21 +54,10 @@ struct LogprobArgs {
     float* entropy;
     float* top_logprob;   // [rows][top]
     long long* top_ids;   // [rows][top]
-    float4* part;         // [2 ctas]: {M, S, T, -} of a piece
-    u64* part_keys;       // [2 ctas][top]
     long long row_stride;
     int rows, vocab, top, row_units;
-    int row_ctas;         // CTAs of a row when there are more CTAs than rows, else 0
+    int row_ctas;         // CTAs of a row: a cluster
 };
-
-// The run of units of CTA b: an equal share of all units, or - when there are several CTAs to
-// a row - of one row's, so that no CTA finishes two pieces.
-__host__ __device__ __forceinline__ long long lp_run(const LogprobArgs& a, int b, int ctas)
-{
-    if (a.row_ctas == 0) return b * ((long long) a.rows * a.row_units) / ctas;
-    const int row = b / a.row_ctas;
-    return (long long) row * a.row_units + (long long) (b - row * a.row_ctas) * a.row_units / a.row_ctas;
-}
 
 __device__ __forceinline__ float lp_ex2(float x)
 {
@@ -270,296 +265,18 @@ __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, float M,
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __grid_constant__ LogprobArgs a)
+// A row of several pieces: part(p) is {M, S, T} of piece p, keys(p) its descending keys.
+template <typename T, typename Part, typename Keys>
+__device__ __forceinline__ void lp_join(const LogprobArgs& a, int row, int pieces, Part part, Keys keys, u64 (*lists)[32])
 {
-    __shared__ u64 lists[kLpWarps][32];
-    __shared__ u64 buffer[kLpBuffer + kLpThreads * kLpVec];
-    __shared__ float red[kLpWarps][3];
-    __shared__ u64 sh_bound;
-    __shared__ int sh_count, sh_cols, cols[kLpThreads];
-    __shared__ int best_vec[kLpThreads];
-    griddep_launch();
-    griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int u = (int) lp_run(a, blockIdx.x, gridDim.x);
-    const int u_end = (int) lp_run(a, blockIdx.x + 1, gridDim.x);
-    while (u < u_end) {
-        const int row = u / a.row_units;
-        const int c0 = u - row * a.row_units, c1 = min(a.row_units, c0 + (u_end - u));  // units of the row: the piece
-        u += c1 - c0;
-        const LpRow<T> r(a, row);
-        const int nv = r.vectors();
-        const int v0 = c0 * kLpThreads + tid, v1 = min(nv, c1 * kLpThreads);  // vectors v0, v0 + 256, ... of this thread
-        float best = -INFINITY, second = -INFINITY, ref = -1e30f;
-        f32x2 s2 = lp_pair(0.f, 0.f), t2 = s2;
-        int bv = v0;
-        // vectors b .. b + n of the row into L2, one request of one thread
-        auto prefetch = [&](int b, int n) {
-            const int lo = max(b, r.inside(0) ? 0 : 1), hi = min(b + n, min(v1, r.end / kLpVec));
-            if (tid == 0 && hi > lo) {
-                const char* p = reinterpret_cast<const char*>(r.p + (long long) lo * kLpVec);
-                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((hi - lo) * kLpVec * (int) sizeof(T)) : "memory");
-            }
-        };
-        auto raise = [&](float cm) {  // before elements of at most cm are added
-            const float c2 = cm * kLpLog2e;
-            if (c2 > ref + kLpSlack) {
-                const float d = ref - c2, k = lp_ex2(d);
-                float s0, s1, t0, t1;
-                lp_unpair(s2, s0, s1);
-                lp_unpair(t2, t0, t1);
-                t2 = lp_pair((t0 + d * s0) * k, (t1 + d * s1) * k);
-                s2 = lp_pair(s0 * k, s1 * k);
-                ref = c2;
-            }
-        };
-        auto rank = [&](float cm, int v) {  // a vector's maximum among this thread's
-            second = fmaxf(second, fminf(best, cm));
-            bv = cm > best ? v : bv;
-            best = fmaxf(best, cm);
-        };
-        auto add = [&](float x0, float x1) {  // finite or NaN
-            const f32x2 y = lp_fma2(lp_pair(x0, x1), lp_pair(kLpLog2e, kLpLog2e), lp_pair(-ref, -ref));
-            float y0, y1;
-            lp_unpair(y, y0, y1);
-            const f32x2 e = lp_pair(lp_ex2(y0), lp_ex2(y1));
-            s2 = lp_add2(s2, e);
-            t2 = lp_fma2(y, e, t2);
-        };
-        auto max8 = [](const float (&f)[8]) {
-            return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        };
-        auto largest = [&](const LpVec<T>& x) {
-            if constexpr (sizeof(T) == 4) {
-                float f[8];
-                x.get(f);
-                return max8(f);
-            } else {
-                const uint4 w = x.w[0];
-                const float2 m = lp_float2<T>(lp_max2<T>(lp_max2<T>(w.x, w.y), lp_max2<T>(w.z, w.w)));
-                return fmaxf(m.x, m.y);
-            }
-        };
-        auto add8 = [&](const LpVec<T>& x) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    const uint4 w = x.w[i >> 1];
-                    add(lp_low(__uint_as_float(i & 1 ? w.z : w.x)), lp_low(__uint_as_float(i & 1 ? w.w : w.y)));
-                } else {
-                    const uint4 w = x.w[0];
-                    const float2 f = lp_float2<T>(lp_low2<T>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w));
-                    add(f.x, f.y);
-                }
-            }
-        };
-        auto take_any = [&](int v) {
-            float f[8];
-            r.read(v, f);
-            const float cm = max8(f);
-            raise(cm);
-            rank(cm, v);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
-        };
-        {
-            constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
-            constexpr int kFar = 2;
-            prefetch(c0 * kLpThreads, kFar * kAhead * kLpThreads);
-            int v = v0;
-            if (v < v1 && !r.inside(v)) {
-                take_any(v);
-                v += kLpThreads;
-            }
-            for (; v + (kAhead - 1) * kLpThreads < v1 && r.inside(v + (kAhead - 1) * kLpThreads); v += kAhead * kLpThreads) {
-                prefetch(v - tid + kFar * kAhead * kLpThreads, kAhead * kLpThreads);
-                LpVec<T> x[kAhead];
-                float cm[kAhead];
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) x[i].load(r.p + (long long) (v + i * kLpThreads) * kLpVec);
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) cm[i] = largest(x[i]);
-                float all = cm[0];
-#pragma unroll
-                for (int i = 1; i < kAhead; ++i) all = fmaxf(all, cm[i]);
-                raise(all);
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    rank(cm[i], v + i * kLpThreads);
-                    add8(x[i]);
-                }
-            }
-            for (; v < v1; v += kLpThreads) take_any(v);
-        }
-        float s, t;
-        {
-            float s1, t1;
-            lp_unpair(s2, s, s1);
-            lp_unpair(t2, t, t1);
-            s += s1;
-            t += t1;
-        }
-
-        // M, S, T of the piece
-        float M = best;
-#pragma unroll
-        for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
-        if (lane == 0) red[warp][0] = M;
-        if (tid == 0) sh_count = sh_cols = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kLpWarps; ++i) M = fmaxf(M, red[i][0]);
-        if (lp_far<T>(M)) {  // logits whose product with log2 e leaves fp32's exact range, as a mask of the type's lowest value
-            s = t = 0.f;
-            for (int v = v0; v < v1; v += kLpThreads) {
-                float f[8];
-                r.read(v, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float y = lp_bound((f[i] - M) * kLpLog2e), e = lp_ex2(y);
-                    s += e;
-                    t = fmaf(y, e, t);
-                }
-            }
-        } else {
-            const float d = ref - M * kLpLog2e, k = s == 0.f ? 0.f : lp_ex2(d);
-            t = s == 0.f ? 0.f : (t + d * s) * k;
-            s *= k;
-        }
-        {
-#pragma unroll
-            for (int i = 16; i; i >>= 1) {
-                s += __shfl_xor_sync(~0u, s, i);
-                t += __shfl_xor_sync(~0u, t, i);
-            }
-            if (lane == 0) red[warp][1] = s, red[warp][2] = t;
-        }
-        u64 key = 0;
-        if (a.top > 0) {
-            float f[8];
-            if (v0 < v1) {
-                r.read(bv, f);
-#pragma unroll
-                for (int i = 7; i >= 0; --i) {
-                    const int e = bv * kLpVec + i;
-                    if (f[i] == best && e >= r.shift && e < r.end) key = lp_key(best, e - r.shift);
-                }
-            }
-            best_vec[tid] = bv;
-            const u64 mine = key;
-            if (a.top == 1) {  // the largest of the threads' largest
-#pragma unroll
-                for (int i = 16; i; i >>= 1) {
-                    const u64 o = __shfl_xor_sync(~0u, key, i);
-                    key = o > key ? o : key;
-                }
-                if (lane == 0) lists[0][warp] = key;
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kLpWarps; ++i) key = lists[0][i] > key ? lists[0][i] : key;
-            } else {
-                key = lp_merge_warps(lp_sort(key, lane), lists, warp, lane);
-                if (warp == 0 && lane == a.top - 1) sh_bound = key;
-                __syncthreads();
-                u64 bound = sh_bound;
-                auto push = [&](const float (&x)[8], int v) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int e = v * kLpVec + i;
-                        if (e >= r.shift && e < r.end) {
-                            const u64 k = lp_key(x[i], e - r.shift);
-                            if (k >= bound) buffer[atomicAdd(&sh_count, 1)] = k;
-                        }
-                    }
-                };
-                // the best vectors of the threads above the bound (at most 32 of them, unless
-                // the piece has fewer threads with elements than alternatives)
-                if (v0 < v1 && mine >= bound) {
-                    push(f, bv);
-                    if (v0 + kLpThreads < v1 && lp_order(second) >= (unsigned) (bound >> 32)) cols[atomicAdd(&sh_cols, 1)] = tid;
-                }
-                __syncthreads();
-                const int units = (v1 - c0 * kLpThreads + kLpThreads - 1) / kLpThreads;  // vectors of a column, at most
-                const int again = sh_cols * units;
-                for (int i0 = 0;; i0 += kLpThreads) {
-                    const int n = sh_count;
-                    __syncthreads();  // every thread has read it
-                    if (n > kLpBuffer) {  // cut back to the best 32, raise the bound
-                        if (warp == 0) {
-                            u64 l = 0;
-                            for (int b = 0; b < n; b += 32) l = lp_merge(l, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
-                            buffer[lane] = l;
-                            if (lane == a.top - 1) sh_bound = l;
-                            if (lane == 0) sh_count = 32;
-                        }
-                        __syncthreads();
-                        bound = sh_bound;
-                    }
-                    if (i0 >= again) break;
-                    if (i0 + tid < again) {
-                        const int col = cols[(i0 + tid) / units];
-                        const int v = c0 * kLpThreads + col + ((i0 + tid) % units) * kLpThreads;
-                        if (v < v1 && v != best_vec[col]) {
-                            float x[8];
-                            r.read(v, x);
-                            push(x, v);
-                        }
-                    }
-                    __syncthreads();
-                }
-                if (warp == 0) {
-                    key = 0;
-                    const int n = sh_count;
-                    for (int b = 0; b < n; b += 32) key = lp_merge(key, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
-                }
-            }
-        }
-        __syncthreads();
-        if (warp == 0) {
-            float S = 0.f, Tt = 0.f;
-#pragma unroll
-            for (int i = 0; i < kLpWarps; ++i) S += red[i][1], Tt += red[i][2];
-            if (c1 - c0 == a.row_units) {
-                lp_write<T>(a, row, M, S, Tt, key, tid);
-            } else {
-                const int piece = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
-                if (lane == 0) a.part[piece] = make_float4(M, S, Tt, 0.f);
-                if (lane < a.top) a.part_keys[(long long) piece * a.top + lane] = key;
-            }
-        }
-        __syncthreads();  // shared memory is free for the next piece
-    }
-}
-
-// The row that begins in the run of CTA b of the first kernel and does not end there
-// (b: this block, or the first CTA of its row).
-template <typename T>
-__global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __grid_constant__ LogprobArgs a, int ctas)
-{
-    __shared__ u64 lists[kLpWarps][32];
-    griddep_launch();
-    griddep_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int cta = a.row_ctas ? blockIdx.x * a.row_ctas : blockIdx.x;
-    int row = blockIdx.x, pieces = a.row_ctas;
-    if (!a.row_ctas) {
-        const long long total = (long long) a.rows * a.row_units;
-        const long long u0 = lp_run(a, cta, ctas), u1 = lp_run(a, cta + 1, ctas);
-        if (u0 == u1) return;
-        row = (int) ((u1 - 1) / a.row_units);  // the run's last row
-        const long long first = (long long) row * a.row_units, last = first + a.row_units - 1;
-        if (first < u0 || last < u1) return;  // began earlier, or ends here
-        pieces = (int) (((last + 1) * ctas - 1) / total) - cta + 1;
-    }
-    auto at = [&](int p) { return p == 0 ? 2 * cta + 1 : 2 * (cta + p); };
     float M = -INFINITY, S = 0.f, Tt = 0.f;
     if (warp == 0) {
-        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, a.part[at(p)].x);
+        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, part(p).x);
 #pragma unroll
         for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
         for (int p = lane; p < pieces; p += 32) {
-            const float4 q = a.part[at(p)];
+            const float4 q = part(p);
             const float d = lp_far<T>(M) ? (q.x - M) * kLpLog2e : q.x * kLpLog2e - M * kLpLog2e, k = lp_ex2(d);
             S += q.y * k;
             Tt += k == 0.f ? 0.f : (q.z + d * q.y) * k;
@@ -575,82 +292,324 @@ __global__ __launch_bounds__(kLpThreads) void exl3_logprobs_join_kernel(const __
         const int n = pieces * a.top;
         for (int b = warp * 32; b < n; b += kLpThreads) {
             const int i = b + lane;
-            u64 k = 0;
-            if (i < n) k = a.part_keys[(long long) at(i / a.top) * a.top + i % a.top];
-            key = lp_merge(key, lp_sort(k, lane), lane);
+            key = lp_merge(key, lp_sort(i < n ? keys(i / a.top)[i % a.top] : 0, lane), lane);
         }
         key = lp_merge_warps(key, lists, warp, lane);
     }
     if (warp == 0) lp_write<T>(a, row, M, S, Tt, key, tid);
 }
 
+template <typename T>
+__global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __grid_constant__ LogprobArgs a)
+{
+    __shared__ u64 lists[kLpWarps][32];
+    __shared__ u64 buffer[kLpBuffer + kLpThreads * kLpVec];
+    __shared__ float red[kLpWarps][3];
+    __shared__ u64 sh_bound;
+    __shared__ int sh_count, sh_cols, cols[kLpThreads];
+    __shared__ int best_vec[kLpThreads];
+    __shared__ float4 sh_part;
+    __shared__ u64 sh_keys[32];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int row = blockIdx.x / a.row_ctas, part = blockIdx.x - row * a.row_ctas;
+    // units of the row: this CTA's piece
+    const int c0 = (int) ((long long) part * a.row_units / a.row_ctas), c1 = (int) ((long long) (part + 1) * a.row_units / a.row_ctas);
+    const LpRow<T> r(a, row);
+    const int nv = r.vectors();
+    const int v0 = c0 * kLpThreads + tid, v1 = min(nv, c1 * kLpThreads);  // vectors v0, v0 + 256, ... of this thread
+    float best = -INFINITY, second = -INFINITY, ref = -1e30f;
+    f32x2 s2 = lp_pair(0.f, 0.f), t2 = s2;
+    int bv = v0;
+    // vectors b .. b + n of the row into L2, one request of one thread
+    auto prefetch = [&](int b, int n) {
+        const int lo = max(b, r.inside(0) ? 0 : 1), hi = min(b + n, min(v1, r.end / kLpVec));
+        if (tid == 0 && hi > lo) {
+            const char* p = reinterpret_cast<const char*>(r.p + (long long) lo * kLpVec);
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((hi - lo) * kLpVec * (int) sizeof(T)) : "memory");
+        }
+    };
+    auto raise = [&](float cm) {  // before elements of at most cm are added
+        const float c2 = cm * kLpLog2e;
+        if (c2 > ref + kLpSlack) {
+            const float d = ref - c2, k = lp_ex2(d);
+            float s0, s1, t0, t1;
+            lp_unpair(s2, s0, s1);
+            lp_unpair(t2, t0, t1);
+            t2 = lp_pair((t0 + d * s0) * k, (t1 + d * s1) * k);
+            s2 = lp_pair(s0 * k, s1 * k);
+            ref = c2;
+        }
+    };
+    auto rank = [&](float cm, int v) {  // a vector's maximum among this thread's
+        second = fmaxf(second, fminf(best, cm));
+        bv = cm > best ? v : bv;
+        best = fmaxf(best, cm);
+    };
+    auto add = [&](float x0, float x1) {  // finite or NaN
+        const f32x2 y = lp_fma2(lp_pair(x0, x1), lp_pair(kLpLog2e, kLpLog2e), lp_pair(-ref, -ref));
+        float y0, y1;
+        lp_unpair(y, y0, y1);
+        const f32x2 e = lp_pair(lp_ex2(y0), lp_ex2(y1));
+        s2 = lp_add2(s2, e);
+        t2 = lp_fma2(y, e, t2);
+    };
+    auto max8 = [](const float (&f)[8]) {
+        return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+    };
+    auto largest = [&](const LpVec<T>& x) {
+        if constexpr (sizeof(T) == 4) {
+            float f[8];
+            x.get(f);
+            return max8(f);
+        } else {
+            const uint4 w = x.w[0];
+            const float2 m = lp_float2<T>(lp_max2<T>(lp_max2<T>(w.x, w.y), lp_max2<T>(w.z, w.w)));
+            return fmaxf(m.x, m.y);
+        }
+    };
+    auto add8 = [&](const LpVec<T>& x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                const uint4 w = x.w[i >> 1];
+                add(lp_low(__uint_as_float(i & 1 ? w.z : w.x)), lp_low(__uint_as_float(i & 1 ? w.w : w.y)));
+            } else {
+                const uint4 w = x.w[0];
+                const float2 f = lp_float2<T>(lp_low2<T>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w));
+                add(f.x, f.y);
+            }
+        }
+    };
+    auto take_any = [&](int v) {
+        float f[8];
+        r.read(v, f);
+        const float cm = max8(f);
+        raise(cm);
+        rank(cm, v);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) add(lp_low(f[i]), lp_low(f[i + 1]));
+    };
+    {
+        constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+        constexpr int kFar = 2;
+        prefetch(c0 * kLpThreads, kFar * kAhead * kLpThreads);
+        int v = v0;
+        if (v < v1 && !r.inside(v)) {
+            take_any(v);
+            v += kLpThreads;
+        }
+        for (; v + (kAhead - 1) * kLpThreads < v1 && r.inside(v + (kAhead - 1) * kLpThreads); v += kAhead * kLpThreads) {
+            prefetch(v - tid + kFar * kAhead * kLpThreads, kAhead * kLpThreads);
+            LpVec<T> x[kAhead];
+            float cm[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) x[i].load(r.p + (long long) (v + i * kLpThreads) * kLpVec);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) cm[i] = largest(x[i]);
+            float all = cm[0];
+#pragma unroll
+            for (int i = 1; i < kAhead; ++i) all = fmaxf(all, cm[i]);
+            raise(all);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                rank(cm[i], v + i * kLpThreads);
+                add8(x[i]);
+            }
+        }
+        for (; v < v1; v += kLpThreads) take_any(v);
+    }
+    float s, t;
+    {
+        float s1, t1;
+        lp_unpair(s2, s, s1);
+        lp_unpair(t2, t, t1);
+        s += s1;
+        t += t1;
+    }
+
+    // M, S, T of the piece
+    float M = best;
+#pragma unroll
+    for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
+    if (lane == 0) red[warp][0] = M;
+    if (tid == 0) sh_count = sh_cols = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kLpWarps; ++i) M = fmaxf(M, red[i][0]);
+    if (lp_far<T>(M)) {  // logits whose product with log2 e leaves fp32's exact range, as a mask of the type's lowest value
+        s = t = 0.f;
+        for (int v = v0; v < v1; v += kLpThreads) {
+            float f[8];
+            r.read(v, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = lp_bound((f[i] - M) * kLpLog2e), e = lp_ex2(y);
+                s += e;
+                t = fmaf(y, e, t);
+            }
+        }
+    } else {
+        const float d = ref - M * kLpLog2e, k = s == 0.f ? 0.f : lp_ex2(d);
+        t = s == 0.f ? 0.f : (t + d * s) * k;
+        s *= k;
+    }
+    {
+#pragma unroll
+        for (int i = 16; i; i >>= 1) {
+            s += __shfl_xor_sync(~0u, s, i);
+            t += __shfl_xor_sync(~0u, t, i);
+        }
+        if (lane == 0) red[warp][1] = s, red[warp][2] = t;
+    }
+    u64 key = 0;
+    if (a.top > 0) {
+        float f[8];
+        if (v0 < v1) {
+            r.read(bv, f);
+#pragma unroll
+            for (int i = 7; i >= 0; --i) {
+                const int e = bv * kLpVec + i;
+                if (f[i] == best && e >= r.shift && e < r.end) key = lp_key(best, e - r.shift);
+            }
+            if (key == 0) {  // NaN alone: an id of the vocabulary all the same
+                const int i = max(r.shift - bv * kLpVec, 0);
+                key = lp_key(__uint_as_float(0x7fffffffu), bv * kLpVec + i - r.shift);
+            }
+        }
+        best_vec[tid] = bv;
+        const u64 mine = key;
+        if (a.top == 1) {  // the largest of the threads' largest
+#pragma unroll
+            for (int i = 16; i; i >>= 1) {
+                const u64 o = __shfl_xor_sync(~0u, key, i);
+                key = o > key ? o : key;
+            }
+            if (lane == 0) lists[0][warp] = key;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kLpWarps; ++i) key = lists[0][i] > key ? lists[0][i] : key;
+        } else {
+            key = lp_merge_warps(lp_sort(key, lane), lists, warp, lane);
+            if (warp == 0 && lane == a.top - 1) sh_bound = key;
+            __syncthreads();
+            u64 bound = sh_bound;
+            auto push = [&](const float (&x)[8], int v) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = v * kLpVec + i;
+                    if (e >= r.shift && e < r.end) {
+                        const u64 k = lp_key(x[i], e - r.shift);
+                        if (k >= bound) buffer[atomicAdd(&sh_count, 1)] = k;
+                    }
+                }
+            };
+            // the best vectors of the threads above the bound (at most 32 of them, unless
+            // the piece has fewer threads with elements than alternatives)
+            if (v0 < v1 && mine >= bound) {
+                push(f, bv);
+                if (v0 + kLpThreads < v1 && lp_order(second) >= (unsigned) (bound >> 32)) cols[atomicAdd(&sh_cols, 1)] = tid;
+            }
+            __syncthreads();
+            const int units = (v1 - c0 * kLpThreads + kLpThreads - 1) / kLpThreads;  // vectors of a column, at most
+            const int again = sh_cols * units;
+            for (int i0 = 0;; i0 += kLpThreads) {
+                const int n = sh_count;
+                __syncthreads();  // every thread has read it
+                if (n > kLpBuffer) {  // cut back to the best 32, raise the bound
+                    if (warp == 0) {
+                        u64 l = 0;
+                        for (int b = 0; b < n; b += 32) l = lp_merge(l, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
+                        buffer[lane] = l;
+                        if (lane == a.top - 1) sh_bound = l;
+                        if (lane == 0) sh_count = 32;
+                    }
+                    __syncthreads();
+                    bound = sh_bound;
+                }
+                if (i0 >= again) break;
+                if (i0 + tid < again) {
+                    const int col = cols[(i0 + tid) / units];
+                    const int v = c0 * kLpThreads + col + ((i0 + tid) % units) * kLpThreads;
+                    if (v < v1 && v != best_vec[col]) {
+                        float x[8];
+                        r.read(v, x);
+                        push(x, v);
+                    }
+                }
+                __syncthreads();
+            }
+            if (warp == 0) {
+                key = 0;
+                const int n = sh_count;
+                for (int b = 0; b < n; b += 32) key = lp_merge(key, lp_sort(b + lane < n ? buffer[b + lane] : 0, lane), lane);
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        float S = 0.f, Tt = 0.f;
+#pragma unroll
+        for (int i = 0; i < kLpWarps; ++i) S += red[i][1], Tt += red[i][2];
+        if (a.row_ctas == 1) {
+            lp_write<T>(a, row, M, S, Tt, key, tid);
+        } else {
+            if (lane == 0) sh_part = make_float4(M, S, Tt, 0.f);
+            sh_keys[lane] = key;
+        }
+    }
+    if (a.row_ctas > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (cluster.block_rank() == 0)
+            lp_join<T>(a, row, a.row_ctas,
+                       [&](int p) { return *cluster.map_shared_rank(&sh_part, p); },
+                       [&](int p) { return (const u64*) cluster.map_shared_rank(sh_keys, p); }, lists);
+        cluster.sync();  // the pieces stay until they are read
+    }
+}
+
 // (a row that does not begin on a 16-byte boundary reaches over one vector more)
 static int lp_row_units(int vocab) { return (int) (((long long) vocab + kLpVec - 1 + kLpUnit - 1) / kLpUnit); }
 
-struct LpSplit {
-    int ctas, row_ctas;
-};
-static LpSplit lp_split(long long rows, int row_units)
-{
-    if (rows < kLpCtas) {
-        const int p = std::min<int>((int) (kLpCtas / rows), row_units);
-        return {(int) rows * p, p};
-    }
-    return {kLpCtas, 0};
-}
-
-template <typename T> static int lp_launch(const LogprobArgs& a, int ctas, cudaStream_t st)
+template <typename T> static int lp_launch(const LogprobArgs& a, cudaStream_t st)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) ctas);
+    cfg.gridDim = dim3((unsigned) (a.rows * a.row_ctas));
     cfg.blockDim = dim3(kLpThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned) a.row_ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, exl3_logprobs_kernel<T>, a) != cudaSuccess) return kErrLaunch;
-    if (a.row_ctas == 1 || (a.row_ctas == 0 && a.rows % ctas == 0)) return kOk;  // no run cuts a row
-    if (a.row_ctas) cfg.gridDim = dim3((unsigned) a.rows);
-    return cudaLaunchKernelEx(&cfg, exl3_logprobs_join_kernel<T>, a, ctas) == cudaSuccess ? kOk : kErrLaunch;
+    cfg.numAttrs = a.row_ctas > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, exl3_logprobs_kernel<T>, a) == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace exl3b200
 
 using namespace exl3b200;
 
-extern "C" size_t exl3b200_token_logprobs_scratch_size(int rows, int vocab, int top)
-{
-    if (rows < 1 || vocab < 1 || vocab > (1 << 30) || top < 0 || top > kLpMaxTop || top > vocab) return 0;
-    const int units = lp_row_units(vocab);
-    if ((long long) rows * units > INT_MAX) return 0;
-    const size_t ctas = (size_t) lp_split(rows, units).ctas;
-    return 2 * ctas * (sizeof(float4) + (size_t) top * sizeof(u64));
-}
-
 extern "C" int exl3b200_token_logprobs(const void* logits, long long row_stride, int rows, int vocab, int dtype,
                                        const long long* tokens, int top, float* logprob, float* entropy,
-                                       float* top_logprobs, long long* top_ids, void* scratch, size_t scratch_bytes,
-                                       void* stream)
+                                       float* top_logprobs, long long* top_ids, void* stream)
 {
-    if (!logits || !tokens || !logprob || !entropy || !scratch || (top > 0 && (!top_logprobs || !top_ids))) return kErrNullPointer;
-    const size_t need = exl3b200_token_logprobs_scratch_size(rows, vocab, top);
-    if (need == 0 || (rows > 1 && row_stride < vocab)) return kErrBadShape;
+    if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return kErrNullPointer;
+    if (rows < 1 || vocab < 1 || vocab > (1 << 30) || top < 0 || top > kLpMaxTop || top > vocab || (rows > 1 && row_stride < vocab))
+        return kErrBadShape;
     if (dtype != EXL3B200_DTYPE_F16 && dtype != EXL3B200_DTYPE_BF16 && dtype != EXL3B200_DTYPE_F32) return kErrBadArgument;
-    if (scratch_bytes < need) return kErrWorkspace;
-    if ((uintptr_t) scratch % 16 || (uintptr_t) logits % (dtype == EXL3B200_DTYPE_F32 ? 4 : 2)) return kErrUnaligned;
+    if ((uintptr_t) logits % (dtype == EXL3B200_DTYPE_F32 ? 4 : 2)) return kErrUnaligned;
     LogprobArgs a = {};
     a.logits = logits, a.tokens = tokens, a.logprob = logprob, a.entropy = entropy;
     a.top_logprob = top_logprobs, a.top_ids = top_ids;
     a.row_stride = row_stride, a.rows = rows, a.vocab = vocab, a.top = top, a.row_units = lp_row_units(vocab);
-    const LpSplit sp = lp_split(rows, a.row_units);
-    const int ctas = sp.ctas;
-    a.row_ctas = sp.row_ctas;
-    a.part = reinterpret_cast<float4*>(scratch);
-    a.part_keys = reinterpret_cast<u64*>(a.part + 2 * ctas);
+    a.row_ctas = std::max(1, std::min({kLpClusterCtas / rows, kLpCluster, a.row_units}));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (dtype == EXL3B200_DTYPE_F16) return lp_launch<__half>(a, ctas, st);
-    if (dtype == EXL3B200_DTYPE_BF16) return lp_launch<__nv_bfloat16>(a, ctas, st);
-    return lp_launch<float>(a, ctas, st);
+    if (dtype == EXL3B200_DTYPE_F16) return lp_launch<__half>(a, st);
+    if (dtype == EXL3B200_DTYPE_BF16) return lp_launch<__nv_bfloat16>(a, st);
+    return lp_launch<float>(a, st);
 }

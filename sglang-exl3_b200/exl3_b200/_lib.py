@@ -183,8 +183,7 @@ SIGNATURES = {
     "exl3b200_rope_append": (_i, [_vp, _vp]),
     "exl3b200_paged_attention_scratch_size": (_sz, [_i, _i, _i, _i]),
     "exl3b200_paged_attention": (_i, [_vp, _vp, _sz, _vp]),
-    "exl3b200_token_logprobs_scratch_size": (_sz, [_i, _i, _i]),
-    "exl3b200_token_logprobs": (_i, [_vp, _ll, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "exl3b200_token_logprobs": (_i, [_vp, _ll, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "exl3b200_read_ranges": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp, _sz, _i, _i, _vp]),
     "exl3b200_moe_state_size": (_sz, [_i, _i, _i, _i]),
     "exl3b200_moe_scratch_size": (_sz, [_i, _i, _i, _i]),

@@ -42,9 +42,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     got = TokenLogprobs(lp, torch.empty_like(lp), lp.new_empty((rows, top)) if top else None,
                         tokens.new_empty((rows, top)) if top else None)
     if rows:
-        n = _lib.lib().exl3b200_token_logprobs_scratch_size(rows, vocab, top)
-        scratch = lp.new_empty(n, dtype=torch.uint8)  # the call's own (a captured graph keeps its own, too)
         _lib.launch("exl3b200_token_logprobs", index, logits.data_ptr(), logits.stride(0), rows, vocab,
-                    _OUT_DTYPES[logits.dtype], tokens.data_ptr(), top, got[0].data_ptr(), got[1].data_ptr(),
-                    got[2].data_ptr() if top else None, got[3].data_ptr() if top else None, scratch.data_ptr(), n)
+                    _OUT_DTYPES[logits.dtype], tokens.data_ptr(), top, lp.data_ptr(), got[1].data_ptr(),
+                    got[2].data_ptr() if top else None, got[3].data_ptr() if top else None)
     return got

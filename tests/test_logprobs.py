@@ -11,7 +11,7 @@ P = 4096  # never dereferenced
 
 def call(**kw):
     a = dict(logits=P, stride=1000, rows=2, vocab=1000, dtype=_lib.DTYPE_BF16, tokens=P, top=5, lp=P, ent=P, tlp=P,
-             ids=P, scratch=P, nbytes=1 << 30, stream=None)
+             ids=P, stream=None)
     a.update(kw)
     return _lib.lib().exl3b200_token_logprobs(*a.values())
 
@@ -19,20 +19,13 @@ def call(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(logits=None), _lib.ENULL), (dict(tokens=None), _lib.ENULL), (dict(lp=None), _lib.ENULL),
     (dict(ent=None), _lib.ENULL), (dict(tlp=None), _lib.ENULL), (dict(ids=None), _lib.ENULL),
-    (dict(scratch=None), _lib.ENULL), (dict(rows=0), _lib.EBADSHAPE), (dict(vocab=0), _lib.EBADSHAPE),
+    (dict(rows=0), _lib.EBADSHAPE), (dict(vocab=0), _lib.EBADSHAPE),
     (dict(top=33), _lib.EBADSHAPE), (dict(top=-1), _lib.EBADSHAPE), (dict(vocab=4, stride=4), _lib.EBADSHAPE),
-    (dict(stride=999), _lib.EBADSHAPE), (dict(rows=2 ** 30, vocab=2 ** 20, stride=2 ** 20), _lib.EBADSHAPE),
-    (dict(dtype=_lib.DTYPE_E4M3), _lib.EBADARG), (dict(nbytes=16), _lib.EWORKSPACE),
-    (dict(scratch=P + 8), _lib.EUNALIGNED), (dict(logits=P + 1), _lib.EUNALIGNED)])
+    (dict(stride=999), _lib.EBADSHAPE), (dict(vocab=2 ** 30 + 1, stride=2 ** 31), _lib.EBADSHAPE),
+    (dict(dtype=_lib.DTYPE_E4M3), _lib.EBADARG), (dict(logits=P + 1), _lib.EUNALIGNED),
+    (dict(logits=P + 2, dtype=_lib.DTYPE_F32), _lib.EUNALIGNED)])
 def test_refusals(kw, code):
     assert call(**kw) == code
-
-
-def test_scratch_size():
-    size = _lib.lib().exl3b200_token_logprobs_scratch_size
-    assert size(1, 128256, 5) > 0 and size(1, 128256, 5) <= size(100, 128256, 5)
-    assert size(1, 10, 11) == 0 and size(0, 10, 1) == 0
-    assert call(nbytes=size(2, 1000, 5) - 1) == _lib.EWORKSPACE
 
 
 def test_cpu_tensors_are_refused():

@@ -118,6 +118,9 @@ def test_rows_without_an_answer(cuda_device):
     assert ((got.top_ids >= 0) & (got.top_ids < 5000)).all()
     assert torch.equal(got.top_ids[1].cpu(), torch.arange(8)) and int(got.top_ids[4, 0]) == 1234
     assert all(len(set(r)) == 8 for r in got.top_ids.tolist())
+    one = LP.token_logprobs(x, tokens, 1)
+    assert ((one.top_ids >= 0) & (one.top_ids < 5000)).all() and int(one.top_ids[1, 0]) == 0
+    assert int(one.top_ids[0, 0]) == int(got.top_ids[0, 0]) and torch.equal(one.logprob[:1], got.logprob[:1])
 
 
 def test_strided_rows_streams_and_graphs(cuda_device):
