@@ -917,7 +917,7 @@ template <int D, typename QT, bool F8>
 __global__ __launch_bounds__(32 * kJoinWarps) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
 {
     constexpr float kRef = weight_ref<typename std::conditional<F8, __half, QT>::type>();
-    constexpr int V = D / 32, kFirst = 4;
+    constexpr int V = D / 32, kFirst = 4, kBatch = 8;
     griddep_launch();
     const int lane = threadIdx.x & 31;
     const int m = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
@@ -963,13 +963,16 @@ __global__ __launch_bounds__(32 * kJoinWarps) void exl3_paged_join_kernel(const 
             }
             i0 = kFirst;
         }
-#pragma unroll 8
-        for (int i = i0; i < n; ++i) {
-            const float ki = __shfl_sync(~0u, k, i);
-            float t[V];
-            load(p0 + i, t);
+        for (int i = i0; i < n; i += kBatch) {  // (past the last piece it is read again, with weight 0)
+            float t[kBatch][V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] += ki * t[e];
+            for (int b = 0; b < kBatch; ++b) load(p0 + min(i + b, n - 1), t[b]);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const float kb = __shfl_sync(~0u, k, (i + b) & 31), ki = i + b < n ? kb : 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] += ki * t[b][e];
+            }
         }
     }
 #pragma unroll
