@@ -604,7 +604,8 @@ EXL3B200_API int exl3b200_rope_append(const exl3b200_rope_append_args* args, voi
  *   out[r, h] = sum_p softmax_p(s_p) v_p,  s_p = cap(scale * q[r, h] . k_p),
  * row r = rows_per_seq * s + j is sequence s's token at position seq_lens[s] - rows_per_seq
  * + j and sees the positions up to its own (causal), of those the last `window` when window
- * is positive.  scale and k_scale are positive.  cap(x) = softcap * tanh(x / softcap), x when softcap is 0.  Position p of
+ * is positive.  scale and k_scale are positive.  cap(x) = softcap * tanh(x / softcap), x when softcap is 0
+ * (a softcap is at least 1e-6).  Position p of
  * sequence s lies in page block_table[s][p / page_size]; entries that no row sees are not
  * read.  A row that sees nothing (an empty sequence) gets zeros and lse -inf.  lse (may be
  * NULL): fp32 [rows][q_heads], the natural logarithm of the sum of exp(s_p).

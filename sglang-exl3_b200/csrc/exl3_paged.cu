@@ -133,6 +133,9 @@ __device__ __forceinline__ void store8_e4m3(void* p, const float (&f)[8], float 
 // then takes 16-element units of a head: elements [a, a+8) and [b, b+8), whose pairs
 // turn together - half-split pairs (i, i + r/2) sit in the two vectors, adjacent pairs
 // inside each.  Units beyond the rotated part, and v, are copied.
+// Bound by HBM: 16384 tokens of 64 + 2 x 8 heads of 128 in fp16 (671 MB) take 115 us,
+// 5.8 TB/s.  Tiles of four tokens (one: 138 us, two: 122, eight: 118) share the angles and
+// the launch; few tokens take one each, to reach every SM (one token: 3.5 us, a launch).
 template <typename IN, typename QO, bool E4M3, int D, bool AHEAD>
 __global__ __launch_bounds__(kAppThreads, AHEAD ? 4 : 5) void exl3_rope_append_kernel(const __grid_constant__ AppendArgs a, int tile,
                                                                        int interleaved)
@@ -400,7 +403,9 @@ template <int UNIT> struct Walk {
             c = 0;
             if (++h == a.kv_heads * a.mblocks) {
                 h = 0;
-                if (++s < a.seqs) sequence(a);
+                // (past the last sequence only if the lengths changed under the kernel: it stays there)
+                s = min(s + 1, a.seqs - 1);
+                sequence(a);
             }
         }
     }
@@ -410,7 +415,17 @@ template <int UNIT> struct Walk {
 // stages of its own (no barrier but at an item's end).  The cache is the MMAs' A operand and
 // the query rows (heads of the group, rows of the sequence) their N, so that 8 heads fill an
 // MMA without padding: S^T = K Q^T, its columns' running maxima and sums, the weights
-// transposed in registers (movmatrix) and O^T = V^T P^T.
+// transposed in registers (movmatrix) and O^T = V^T P^T.  (The query rows as the MMA's M,
+// padded to 16, took 459 us instead of 397 for the first size below.)
+//
+// Every position is read once for all query rows of a kv head, by 16-byte asynchronous
+// copies three stages deep; pages are looked up a stage ahead.  Bound by HBM where the cache
+// is large: 64 sequences of up to 16384 (2.69 GB, bf16, 64 / 8 heads of 128) take 397 us with
+// the join, 6.8 TB/s.  With e4m3 caches or 64-wide heads half the bytes carry the same
+// instructions: 16 x 16384 e4m3, 32 / 4 heads, 52 us, 5.2 TB/s.  40 query rows (5 rows of 8
+// heads) hold 160 accumulators a thread: two warps a scheduler, issue-bound at 2.4 TB/s
+// (111 us; as two items of 20 rows, the cache read twice: 114 us).  Small batches are a
+// chain of latencies: 1 x 2049, 64 / 8 heads, 12 us in two kernels.
 template <int D, typename QT, bool F8, int NT>
 __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
 {
@@ -422,7 +437,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     constexpr bool kLo = !(F8 && std::is_same<QT, __nv_bfloat16>::value);
     constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
     constexpr bool kQShared = NT > 2;
-    constexpr int kBlocks = S::kPos == 32 && NT <= 2 ? 2 : 1;  // 16-position blocks of a step
+    constexpr int kBlocks = S::kPos == 32 && NT <= 3 ? 2 : 1;  // 16-position blocks of a step (e4m3, 24 rows: 78.5 -> 68.5 us for 16 x 16384)
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
     __shared__ __align__(8) float sh_rs[kRowScale ? 8 * NT : 1];
@@ -451,7 +466,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     }
     u0 = (int) ((long long) blockIdx.x * total / grid);
     u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
-    for (int base = 0, s0 = 0;; s0 += 32) {
+    for (int base = 0, s0 = 0; s0 < a.seqs; s0 += 32) {
         w.s = s0 + lane;
         int n = 0;
         if (w.s < a.seqs) {
@@ -475,6 +490,11 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             break;
         }
         base += __shfl_sync(~0u, inc, 31);
+        if (s0 + 32 >= a.seqs) {  // (only if the lengths changed under the kernel)
+            w.s = a.seqs - 1;
+            w.sequence(a);
+            w.h = w.c = 0;
+        }
     }
 
     const unsigned ring = (unsigned) __cvta_generic_to_shared(smem) + warp * (kStages * S::kSlot);
@@ -718,16 +738,20 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 return t;
             };
             const bool capped = a.softcap > 0.f;
-            if (capped) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + exp(2 x / cap)))
-                const float capl = a.softcap * kLog2e, icap = 2.f / a.softcap;
+            if (capped) {
+                // cap tanh(t), t = x / cap: cap (1 - 2 / (1 + exp(2 t))), near 0 (where that cancels) x (1 - t^2 / 3 + 2 t^4 / 15)
+                const float capl = a.softcap * kLog2e, icap = 2.f / a.softcap, tcap = kLn2 / a.softcap;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const float2 t = factor(nt);
+                    const float2 f = factor(nt);
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[b][nt][i] = fmaf(-2.f * capl, rcp(1.f + ex2(s[b][nt][i] * ((i & 1) ? t.y : t.x) * icap)), capl);
+                        for (int i = 0; i < 4; ++i) {
+                            const float y = s[b][nt][i] * ((i & 1) ? f.y : f.x), t = y * tcap, t2 = t * t;
+                            const float far = fmaf(-2.f * capl, rcp(1.f + ex2(y * icap)), capl);
+                            s[b][nt][i] = fabsf(t) < 0.06f ? y * fmaf(t2, fmaf(t2, 2.f / 15.f, -1.f / 3.f), 1.f) : far;
+                        }
                 }
             }
             if (!open) {
@@ -912,7 +936,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 int pieces = 0;
                 if (starts && !whole) {
                     const long long last = (long long) u + (w.n - 1 - w.c);  // the item's last unit
-                    pieces = (int) (((last + 1) * grid - 1) / total) - (int) blockIdx.x + 1;
+                    pieces = min((int) (((last + 1) * grid - 1) / total), grid - 1) - (int) blockIdx.x + 1;
                 }
                 a.desc[blockIdx.x] = make_int4(w.s, w.h, pieces, 0);
             }
@@ -926,7 +950,8 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 // Joins the pieces of the items that the CTAs' runs split: block (x, y) takes the item that
 // begins in the run of CTA x and its rows 8y .. 8y + 7, a warp each, in the order of the
 // pieces (so that a result does not depend on timing).  A chain of loads: the first pieces
-// are read along with the descriptor that says how many there are.
+// are read along with the descriptor that says how many there are, the others eight at a
+// time (1 x 2049, 33 pieces: 14.1 -> 12.0 us for both kernels).
 constexpr int kJoinWarps = 8;
 template <int D, typename QT, bool F8>
 __global__ __launch_bounds__(32 * kJoinWarps) void exl3_paged_join_kernel(const __grid_constant__ AttnArgs a)
@@ -1178,7 +1203,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     if (need == 0) return kErrBadShape;
     if (p->dtype != kF16 && p->dtype != kBf16) return kErrBadArgument;
     if (c.dtype != kE4m3 && c.dtype != p->dtype) return kErrBadArgument;
-    if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap) || !(p->scale > 0.f) || !std::isfinite(p->scale)) return kErrBadArgument;
+    if (!(p->softcap == 0.f || p->softcap >= 1e-6f) || !std::isfinite(p->softcap) || !(p->scale > 0.f) || !std::isfinite(p->scale)) return kErrBadArgument;
     if (scratch_bytes < need) return kErrWorkspace;
     if (misaligned(scratch, 256) || misaligned(p->q, 16) || misaligned(p->out, 16)) return kErrUnaligned;
     if (p->q_stride % 8 || p->q_head_stride % 8 || p->out_stride % 8 || p->out_head_stride % 8) return kErrUnaligned;
@@ -1207,7 +1232,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     while (l < 31 && (1u << l) < (unsigned) c.page_size) ++l;
     a.page_mul = (unsigned) ((((1ull << l) - (unsigned) c.page_size) << 32) / (unsigned) c.page_size + 1);
     a.page_sh1 = std::min(l, 1), a.page_sh2 = std::max(l - 1, 0);
-    a.window = p->window, a.scale = p->scale, a.softcap = p->softcap;
+    a.window = p->window >= capacity ? 0 : p->window, a.scale = p->scale, a.softcap = p->softcap;
     a.status = exl3_status_dev_ptr();
     if (!a.status) return kErrLaunch;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -163,8 +163,8 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         raise RuntimeError("q must have rows_per_seq rows for each sequence, block_table a column")
     if heads < 1 or heads % kv_heads or R * (heads // kv_heads) > _lib.PAGED_MAX_ROWS:
         raise RuntimeError(f"q_heads must be a multiple of kv_heads, rows_per_seq * group at most {_lib.PAGED_MAX_ROWS}")
-    if window < 0 or not 0.0 <= softcap < float("inf"):
-        raise RuntimeError("window and softcap must not be negative")
+    if window < 0 or not (softcap == 0.0 or 1e-6 <= softcap < float("inf")):
+        raise RuntimeError("window must not be negative, softcap 0 or at least 1e-6")
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise RuntimeError("scale must be positive")

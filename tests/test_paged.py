@@ -67,7 +67,7 @@ def test_append_refusals(kw, code):
     (dict(table_stride=3), _lib.EBADSHAPE), (dict(window=-1), _lib.EBADSHAPE), (dict(q_heads=7), _lib.EBADSHAPE),
     (dict(q_heads=1), _lib.EBADSHAPE), (dict(rows_per_seq=0), _lib.EBADSHAPE),
     (dict(rows_per_seq=257), _lib.EBADSHAPE), (dict(dtype=_lib.DTYPE_F32), _lib.EBADARG),
-    (dict(softcap=-1.0), _lib.EBADARG), (dict(softcap=float("nan")), _lib.EBADARG),
+    (dict(softcap=-1.0), _lib.EBADARG), (dict(softcap=float("nan")), _lib.EBADARG), (dict(softcap=1e-9), _lib.EBADARG),
     (dict(scale=float("inf")), _lib.EBADARG), (dict(scale=0.0), _lib.EBADARG), (dict(scale=-0.1), _lib.EBADARG), (dict(nbytes=4096), _lib.EWORKSPACE),
     (dict(scratch=4096 + 16), _lib.EUNALIGNED), (dict(q=P + 8), _lib.EUNALIGNED),
     (dict(q_stride=1023), _lib.EUNALIGNED), (dict(out_head_stride=130), _lib.EUNALIGNED),

@@ -137,6 +137,11 @@ CASES = [
     ([1000, 129, 40], 16, 2, 64, FP16, FP16, 16, 1, 100, 0.0),
     ([1000, 129, 40, 3], 16, 2, 128, BF16, E4M3, 24, 4, 65, 20.0),
     ([4097, 1, 2050, 33], 64, 8, 128, BF16, BF16, 16, 1, 2048, 0.0),
+    ([300, 0, 3, 40], 16, 2, 128, BF16, BF16, 16, 5, 2 ** 31 - 1, 0.0),  # a window of everything
+    ([300, 17], 16, 2, 64, FP16, FP16, 16, 1, 0, 1e5),       # a cap far above the scores: they stay as they are
+    ([300, 17], 16, 2, 64, FP16, FP16, 16, 1, 0, 0.5),       # and far below
+    ([1000, 200, 33], 24, 1, 128, BF16, E4M3, 16, 1, 0, 0.0),  # three tiles of rows
+    ([1000, 200, 33], 24, 1, 64, FP16, FP16, 16, 1, 0, 30.0),
     ([17] * 130, 8, 4, 64, BF16, BF16, 16, 1, 0, 0.0),       # more sequences than threads of a CTA
     ([40] * 300, 16, 4, 128, FP16, FP16, 16, 1, 0, 0.0),     # more items than CTAs
 ]
@@ -151,6 +156,7 @@ def test_attention_matches_definition(cuda_device, lens, heads, hk, dim, qt, ct,
     keep = torch.zeros(k.shape[:2], dtype=torch.bool, device=cuda_device)
     for s, ln in enumerate(lens):
         first = max(0, ln - R + 1 - window) if window else 0
+        assert 0 <= first <= ln
         for p in range(first, ln):
             keep[int(table[s, p // page]), p % page] = True
         if window:  # pages wholly before the window may have been given back
@@ -476,6 +482,6 @@ def test_python_refusals(cuda_device):
     for kw in (dict(q=q.half()), dict(q=q.float()), dict(q=q[:, :7]), dict(q=q[:2]), dict(rows_per_seq=2), dict(rows_per_seq=0),
                dict(block_table=table.long()), dict(block_table=table[0]), dict(block_table=table[:, :0]),
                dict(seq_lens=lens.long()), dict(seq_lens=lens[:2]), dict(softcap=-1.0), dict(window=-1),
-               dict(softcap=float("inf")), dict(scale=0.0), dict(scale=-1.0), dict(out=q.half()), dict(out=q[:2]), dict(seq_lens=lens.cpu())):
+               dict(softcap=float("inf")), dict(softcap=1e-7), dict(scale=0.0), dict(scale=-1.0), dict(out=q.half()), dict(out=q[:2]), dict(seq_lens=lens.cpu())):
         with pytest.raises(RuntimeError):
             paged.attention(**{**ok_b, **kw})
