@@ -28,12 +28,6 @@ _CACHE = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.
 _E4M3 = torch.float8_e4m3fn
 
 
-def _on(index: int, *tensors: Optional[torch.Tensor]) -> None:
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise RuntimeError("paged tensors must share a CUDA device")
-
-
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor],
            v_scale: Optional[torch.Tensor]) -> tuple:
     """The fields of ``exl3b200_paged_cache``."""
@@ -44,35 +38,50 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch
         raise RuntimeError("caches must be fp16, bf16 or float8_e4m3fn [pages, page_size, kv_heads, 64 or 128]")
     if v_cache.dtype != dtype or v_cache.shape != shape or v_cache.stride() != strides:
         raise RuntimeError("k and v caches must have the same type, shape and strides")
-    if strides[3] != 1:
-        raise RuntimeError("caches must have unit stride in their last dimension")
     pages, page_size, kv_heads, dim = shape
+    s0, s1, s2, s3 = strides
+    if s3 != 1:
+        raise RuntimeError("caches must have unit stride in their last dimension")
     if not (pages and page_size and kv_heads):
         raise RuntimeError("caches must not be empty")
-    st = [s if n > 1 else 0 for s, n in zip(strides, shape)]
-    if (pages > 1 and not st[0]) or (page_size > 1 and not st[1]) or (kv_heads > 1 and not st[2]):
+    if pages == 1:
+        s0 = 0
+    if page_size == 1:
+        s1 = 0
+    if kv_heads == 1:
+        s2 = 0
+    if (pages > 1 and not s0) or (page_size > 1 and not s1) or (kv_heads > 1 and not s2):
         raise RuntimeError("caches must not be expanded views")
-    scales = [0, 0]
-    for i, s in enumerate((k_scale, v_scale)):
-        if s is not None:
-            if dtype != _E4M3:
-                raise RuntimeError("k_scale and v_scale belong to float8_e4m3fn caches")
-            if s.dtype != torch.float32 or s.numel() != kv_heads or not s.is_contiguous():
-                raise RuntimeError("k_scale and v_scale must be contiguous fp32 [kv_heads]")
-            scales[i] = s.data_ptr()
-    return (k_cache.data_ptr(), v_cache.data_ptr(), _CACHE[dtype], pages, page_size, kv_heads, dim, st[0], st[1], st[2],
-            scales[0], scales[1])
+    ks = vs = 0
+    if k_scale is not None:
+        ks = _scale(k_scale, dtype, kv_heads)
+    if v_scale is not None:
+        vs = _scale(v_scale, dtype, kv_heads)
+    return (k_cache.data_ptr(), v_cache.data_ptr(), _CACHE[dtype], pages, page_size, kv_heads, dim, s0, s1, s2, ks, vs)
 
 
-def _aligned(t: torch.Tensor) -> bool:
+def _scale(s: torch.Tensor, dtype: torch.dtype, kv_heads: int) -> int:
+    if dtype != _E4M3:
+        raise RuntimeError("k_scale and v_scale belong to float8_e4m3fn caches")
+    if s.dtype != torch.float32 or s.numel() != kv_heads or not s.is_contiguous():
+        raise RuntimeError("k_scale and v_scale must be contiguous fp32 [kv_heads]")
+    return s.data_ptr()
+
+
+def _device(index: int, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError("paged tensors must share a CUDA device")
+
+
+def _rows(t: torch.Tensor, copy: bool = True):
+    """An input [rows, heads, head_dim] whose heads begin on 16-byte boundaries (itself, or a
+    copy), its address and its row and head strides; None where it is not and may not be copied."""
     s0, s1, s2 = t.stride()
-    step = 4 if t.dtype == torch.float32 else 8  # elements of 16 bytes
-    return s2 == 1 and (s0 | s1) % step == 0 and t.data_ptr() % 16 == 0
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """An input [rows, heads, head_dim] whose heads begin on 16-byte boundaries: itself, or a copy."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+    p = t.data_ptr()
+    if s2 != 1 or (s0 | s1) % (4 if t.dtype == torch.float32 else 8) or p % 16:
+        return _rows(t.clone(memory_format=torch.contiguous_format), False) if copy else None
+    return t, p, s0, s1
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -91,7 +100,10 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     in the cache's type, bf16 for an e4m3 cache) may be ``q``."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     index = k_cache.get_device()
-    _on(index, v_cache, q, k, v, positions, slots, inv_freq, q_out, k_scale, v_scale)
+    if not (q.get_device() == k.get_device() == v.get_device() == positions.get_device() == slots.get_device()
+            == inv_freq.get_device() == index):
+        raise RuntimeError("paged tensors must share a CUDA device")
+    _device(index, v_cache, q_out, k_scale, v_scale)
     src, cache = q.dtype, k_cache.dtype
     if src not in _IN or k.dtype != src or v.dtype != src:
         raise RuntimeError("q, k and v must be of one type: fp16, bf16 or fp32")
@@ -99,7 +111,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     if len(shape) != 3 or shape[2] != c[6]:
         raise RuntimeError("q must be [tokens, q_heads, head_dim]")
     tokens, heads, dim = shape
-    if k.shape != (tokens, c[5], dim) or v.shape != (tokens, c[5], dim):
+    if k.shape != (tokens, c[5], dim) or v.shape != k.shape:
         raise RuntimeError("k and v must be [tokens, kv_heads, head_dim]")
     if (positions.dtype != torch.int64 or slots.dtype != torch.int64 or positions.shape != (tokens,)
             or slots.shape != (tokens,)):
@@ -113,15 +125,17 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
         raise RuntimeError("q_out must be fp16 or bf16, shaped like q")
     elif cache != _E4M3 and q_out.dtype != cache:
         raise RuntimeError("q_out must have the cache's type")
-    elif not _aligned(q_out):
-        raise RuntimeError("q_out's heads must begin on 16-byte boundaries with unit stride")
     if tokens == 0 or heads == 0:
         return q_out
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = _rows(q_out, copy=False)
+    if out is None:
+        raise RuntimeError("q_out's heads must begin on 16-byte boundaries with unit stride")
+    q, qp, q0, q1 = _rows(q)
+    k, kp, k0, k1 = _rows(k)
+    v, vp, v0, v1 = _rows(v)
     positions, slots, inv_freq = positions.contiguous(), slots.contiguous(), inv_freq.contiguous()
-    args = _lib.pack_rope_append(*c, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), positions.data_ptr(),
-                                 slots.data_ptr(), inv_freq.data_ptr(), *q.stride()[:2], *k.stride()[:2],
-                                 *v.stride()[:2], *q_out.stride()[:2], tokens, heads, rotary, int(bool(interleaved)),
+    args = _lib.pack_rope_append(*c, qp, kp, vp, out[1], positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(),
+                                 q0, q1, k0, k1, v0, v1, out[2], out[3], tokens, heads, rotary, bool(interleaved),
                                  _IN[src], _IN[q_out.dtype])
     _lib.launch("exl3b200_rope_append", index, args)
     return q_out
@@ -146,7 +160,9 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     ``out`` (q's type), with ``return_lse`` also fp32 ``lse [rows, q_heads]``."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     index = k_cache.get_device()
-    _on(index, v_cache, q, block_table, seq_lens, k_scale, v_scale, out)
+    if not q.get_device() == block_table.get_device() == seq_lens.get_device() == index:
+        raise RuntimeError("paged tensors must share a CUDA device")
+    _device(index, v_cache, k_scale, v_scale, out)
     dtype, shape = q.dtype, q.shape
     if dtype not in (torch.float16, torch.bfloat16) or len(shape) != 3 or shape[2] != c[6]:
         raise RuntimeError("q must be fp16 or bf16 [rows, q_heads, head_dim]")
@@ -170,18 +186,18 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         raise RuntimeError("scale must be positive")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype != dtype or not _aligned(out):
+    elif out.shape != shape or out.dtype != dtype or _rows(out, copy=False) is None:
         raise RuntimeError("out must be shaped like q, of its type, heads on 16-byte boundaries with unit stride")
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if rows:
-        q = _rows(q)
+        q, qp, q0, q1 = _rows(q)
+        _, op, o0, o1 = _rows(out, copy=False)
         n = _lib.lib().exl3b200_paged_attention_scratch_size(R, heads, kv_heads, dim)
         # the scratch is the call's own (a captured graph keeps its own, too)
         scratch = q.new_empty(n, dtype=torch.uint8)
-        args = _lib.pack_paged_attention(*c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                                         block_table.data_ptr(), seq_lens.data_ptr(), *q.stride()[:2],
-                                         *out.stride()[:2], block_table.stride(0) if seqs > 1 else max_pages, seqs, R,
-                                         heads, max_pages, min(window, 2 ** 31 - 1), _IN[dtype],
-                                         scale, softcap)
+        args = _lib.pack_paged_attention(*c, qp, op, lse.data_ptr() if return_lse else 0, block_table.data_ptr(),
+                                         seq_lens.data_ptr(), q0, q1, o0, o1,
+                                         block_table.stride(0) if seqs > 1 else max_pages, seqs, R, heads, max_pages,
+                                         min(window, 2 ** 31 - 1), _IN[dtype], scale, softcap)
         _lib.launch("exl3b200_paged_attention", index, args, scratch.data_ptr(), n)
     return (out, lse) if return_lse else out
