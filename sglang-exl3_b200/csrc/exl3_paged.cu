@@ -390,26 +390,27 @@ template <int D, bool F8> struct AttnShape {
 // the sequence's visible positions).  Every CTA owns a contiguous run of units.
 template <int UNIT> struct Walk {
     int s, h, c, n, c0, lo, len;
-    __device__ __forceinline__ void sequence(const AttnArgs& a)
+    // `tokens`: the sequence's length, cut to what its pages hold
+    __device__ __forceinline__ void sequence(const AttnArgs& a, int tokens)
     {
-        len = min(max(__ldg(a.lens + s), 0), a.capacity);
+        len = tokens;
         lo = a.window > 0 ? max(0, len - a.rows + 1 - a.window) : 0;
         c0 = lo / UNIT;
         n = max(1, (len + UNIT - 1) / UNIT - c0);  // a sequence without tokens has one (masked) unit: its rows are written too
     }
-    __device__ __forceinline__ void next(const AttnArgs& a)
+    template <typename Length> __device__ __forceinline__ void next(const AttnArgs& a, Length length)
     {
         if (++c == n) {
             c = 0;
             if (++h == a.kv_heads * a.mblocks) {
                 h = 0;
-                // (past the last sequence only if the lengths changed under the kernel: it stays there)
-                s = min(s + 1, a.seqs - 1);
-                sequence(a);
+                s = min(s + 1, a.seqs - 1);  // (past the last sequence: nothing follows)
+                sequence(a, length(s));
             }
         }
     }
 };
+__device__ __forceinline__ int attn_length(const AttnArgs& a, int s) { return min(max(__ldg(a.lens + s), 0), a.capacity); }
 
 // One CTA: its run of units, warp w the positions w * kPos .. of each, through a ring of
 // stages of its own (no barrier but at an item's end).  The cache is the MMAs' A operand and
@@ -440,6 +441,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     constexpr int kBlocks = S::kPos == 32 && NT <= 3 ? 2 : 1;  // 16-position blocks of a step (e4m3, 24 rows: 78.5 -> 68.5 us for 16 x 16384)
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
+    __shared__ int sh_start[3], sh_len[32 * kAttnWarps];
     __shared__ __align__(8) float sh_rs[kRowScale ? 8 * NT : 1];
     __shared__ long long sh_q[8 * NT];                // the item's rows: offset in q,
     __shared__ int sh_out[8 * NT];                    // row * q_heads + head,
@@ -450,52 +452,61 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     const int g = lane >> 2, c = lane & 3;
     const int items = a.kv_heads * a.mblocks;  // of a sequence
 
-    // units of all sequences, and where this CTA's run begins (every warp for itself)
+    // Units of all sequences, and where this CTA's run begins: by the first warp, and the
+    // lengths from there on through a window in shared memory, so that the warps never differ
+    // about where an item ends - not even if a caller wrongly changes lengths under the kernel.
     Walk<S::kUnit> w;
-    int total = 0, grid, u0, u1;
-    for (w.s = lane; w.s < a.seqs; w.s += 32) {
-        w.sequence(a);
-        total += w.n * items;
-        if (blockIdx.x == 0 && warp == 0 && __ldg(a.lens + w.s) > a.capacity) atomicCAS(a.status, 0, (int) kErrBadArgument);
+    if (warp == 0) {
+        int total = 0;
+        for (w.s = lane; w.s < a.seqs; w.s += 32) {
+            w.sequence(a, attn_length(a, w.s));
+            total += w.n * items;
+            if (blockIdx.x == 0 && __ldg(a.lens + w.s) > a.capacity) atomicCAS(a.status, 0, (int) kErrBadArgument);
+        }
+        total = __reduce_add_sync(~0u, total);
+        const int grid = min((int) gridDim.x, total);
+        const int u0 = (int) ((long long) blockIdx.x * total / grid);
+        int first = a.seqs - 1, in = 0;
+        for (int base = 0, s0 = 0; s0 < a.seqs && (int) blockIdx.x < grid; s0 += 32) {
+            w.s = s0 + lane;
+            int n = 0;
+            if (w.s < a.seqs) {
+                w.sequence(a, attn_length(a, w.s));
+                n = w.n * items;
+            }
+            int inc = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int t = __shfl_up_sync(~0u, inc, d);
+                if (lane >= d) inc += t;
+            }
+            const unsigned past = __ballot_sync(~0u, u0 < base + inc);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                first = s0 + l;
+                in = u0 - base - __shfl_sync(~0u, inc - n, l);
+                break;
+            }
+            base += __shfl_sync(~0u, inc, 31);
+        }
+        if (lane == 0) sh_start[0] = total, sh_start[1] = first, sh_start[2] = in;
     }
-    total = __reduce_add_sync(~0u, total);
-    grid = min((int) gridDim.x, total);
+    __syncthreads();
+    const int total = sh_start[0], grid = min((int) gridDim.x, total);
     if ((int) blockIdx.x >= grid) {
         if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
-    u0 = (int) ((long long) blockIdx.x * total / grid);
-    u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
-    for (int base = 0, s0 = 0; s0 < a.seqs; s0 += 32) {
-        w.s = s0 + lane;
-        int n = 0;
-        if (w.s < a.seqs) {
-            w.sequence(a);
-            n = w.n * items;
-        }
-        int inc = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int t = __shfl_up_sync(~0u, inc, d);
-            if (lane >= d) inc += t;
-        }
-        const unsigned past = __ballot_sync(~0u, u0 < base + inc);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            w.s = s0 + l;
-            const int in = u0 - base - __shfl_sync(~0u, inc - n, l);
-            w.sequence(a);
-            w.h = in / w.n;
-            w.c = in - w.h * w.n;
-            break;
-        }
-        base += __shfl_sync(~0u, inc, 31);
-        if (s0 + 32 >= a.seqs) {  // (only if the lengths changed under the kernel)
-            w.s = a.seqs - 1;
-            w.sequence(a);
-            w.h = w.c = 0;
-        }
-    }
+    const int u0 = (int) ((long long) blockIdx.x * total / grid), u1 = (int) ((long long) (blockIdx.x + 1) * total / grid);
+    w.s = sh_start[1];
+    int len_base = w.s;  // the window's first sequence
+    auto read_lengths = [&] { sh_len[tid] = attn_length(a, min(len_base + tid, a.seqs - 1)); };
+    auto length = [&](int s) { return sh_len[s - len_base]; };
+    read_lengths();
+    __syncthreads();
+    w.sequence(a, length(w.s));
+    w.h = min(sh_start[2] / w.n, items - 1);
+    w.c = min(sh_start[2] - w.h * w.n, w.n - 1);
 
     const unsigned ring = (unsigned) __cvta_generic_to_shared(smem) + warp * (kStages * S::kSlot);
     const unsigned qsh = (unsigned) __cvta_generic_to_shared(smem) + kAttnWarps * kStages * S::kSlot;
@@ -550,7 +561,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
     auto fill = [&](int slot) {
         if (fu < u1) {
             const Walk<S::kUnit> x = f;
-            f.next(a);
+            f.next(a, length);
             const int next = ++fu < u1 ? page_of(f) : -1;
             stage(x, slot, page);
             page = next;
@@ -942,7 +953,13 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             }
             fresh = true;
         }
-        w.next(a);
+        w.next(a, length);
+        if (fresh && w.s - len_base >= 16 * kAttnWarps) {  // half of the window is behind (f is two units ahead at most)
+            __syncthreads();
+            len_base = w.s;
+            read_lengths();
+            __syncthreads();
+        }
         slot = slot == kStages - 1 ? 0 : slot + 1;
     }
 }

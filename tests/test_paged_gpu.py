@@ -171,6 +171,30 @@ def test_attention_matches_definition(cuda_device, lens, heads, hk, dim, qt, ct,
     assert ops.device_status(cuda_device) == 0
 
 
+@pytest.mark.parametrize("seqs", [20011, 50000])
+def test_attention_many_short_sequences(cuda_device, seqs):
+    """Far more sequences than a CTA keeps lengths of: a sequence of one token answers with its
+    value exactly, an empty one with zeros, and a long one among them with the definition's."""
+    gen = torch.Generator(device=cuda_device)
+    gen.manual_seed(seqs)
+    pages = seqs + 700
+    k, v = make_cache(pages, 1, 1, 64, BF16, gen, cuda_device)
+    table = torch.full((seqs, 600), -1, dtype=torch.int32, device=cuda_device)
+    order = torch.randperm(pages, generator=gen, device=cuda_device).int()
+    table[:, 0] = order[:seqs]
+    table[7777, 1:] = order[seqs:seqs + 599]
+    lens = torch.randint(0, 2, (seqs,), generator=gen, device=cuda_device, dtype=torch.int32)
+    lens[7777] = 600
+    q = torch.randn(seqs, 1, 64, generator=gen, device=cuda_device).to(BF16)
+    out, lse = paged.attention(q, k, v, table, lens, return_lse=True)
+    want = torch.where((lens > 0)[:, None], v[table[:, 0].long(), 0, 0], torch.zeros((), dtype=BF16, device=cuda_device))
+    rest = torch.arange(seqs, device=cuda_device) != 7777
+    assert torch.equal(out[rest, 0], want[rest])
+    assert torch.equal(torch.isinf(lse[:, 0]), lens == 0)
+    ref = attention_oracle(q[7777:7778], k, v, table[7777:7778], [600], 1, 0.125, 0.0, 0, None, None)
+    check_attention(out[7777:7778], lse[7777:7778], *ref, 64, BF16)
+
+
 def test_attention_strided_inputs_and_head_major_pool(cuda_device):
     """q a slice of a fused q/k/v output, the pool [pages, kv_heads, page, dim], out a slice,
     the block table a slice of a wider one."""
