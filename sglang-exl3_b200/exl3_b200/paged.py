@@ -15,6 +15,7 @@ whole batch; these operators serve batches whose sequences differ, around the EX
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -72,6 +73,11 @@ def _device(index: int, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise RuntimeError("paged tensors must share a CUDA device")
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_size(rows_per_seq: int, heads: int, kv_heads: int, dim: int) -> int:
+    return _lib.lib().exl3b200_paged_attention_scratch_size(rows_per_seq, heads, kv_heads, dim)
 
 
 def _rows(t: torch.Tensor, copy: bool = True):
@@ -192,7 +198,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     if rows:
         q, qp, q0, q1 = _rows(q)
         _, op, o0, o1 = _rows(out, copy=False)
-        n = _lib.lib().exl3b200_paged_attention_scratch_size(R, heads, kv_heads, dim)
+        n = _scratch_size(R, heads, kv_heads, dim)
         # the scratch is the call's own (a captured graph keeps its own, too)
         scratch = q.new_empty(n, dtype=torch.uint8)
         args = _lib.pack_paged_attention(*c, qp, op, lse.data_ptr() if return_lse else 0, block_table.data_ptr(),
