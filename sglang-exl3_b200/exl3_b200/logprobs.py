@@ -38,11 +38,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     tokens = tokens.contiguous()
-    lp = logits.new_empty(rows, dtype=torch.float32)
-    got = TokenLogprobs(lp, torch.empty_like(lp), lp.new_empty((rows, top)) if top else None,
-                        tokens.new_empty((rows, top)) if top else None)
+    lp, entropy = torch.empty_like(tokens, dtype=torch.float32), torch.empty_like(tokens, dtype=torch.float32)
+    top_ids = top_lp = None
+    if top:
+        top_ids = tokens.new_empty((rows, top))
+        top_lp = torch.empty_like(top_ids, dtype=torch.float32)
     if rows:
         _lib.launch("exl3b200_token_logprobs", index, logits.data_ptr(), logits.stride(0), rows, vocab,
-                    _OUT_DTYPES[logits.dtype], tokens.data_ptr(), top, lp.data_ptr(), got[1].data_ptr(),
-                    got[2].data_ptr() if top else None, got[3].data_ptr() if top else None)
-    return got
+                    _OUT_DTYPES[logits.dtype], tokens.data_ptr(), top, lp.data_ptr(), entropy.data_ptr(),
+                    top_lp.data_ptr() if top else None, top_ids.data_ptr() if top else None)
+    return TokenLogprobs(lp, entropy, top_lp, top_ids)

@@ -126,7 +126,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     if inv_freq.dtype != torch.float32 or rotary > dim or rotary % 16:
         raise RuntimeError("inv_freq must be fp32 with half of the rotated dims, a multiple of 8 up to head_dim / 2")
     if q_out is None:
-        q_out = q.new_empty(shape, dtype=torch.bfloat16 if cache == _E4M3 else cache)
+        q_out = torch.empty_like(q, dtype=torch.bfloat16 if cache == _E4M3 else cache,
+                                 memory_format=torch.contiguous_format)
     elif q_out.shape != shape or q_out.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("q_out must be fp16 or bf16, shaped like q")
     elif cache != _E4M3 and q_out.dtype != cache:
@@ -192,12 +193,15 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         raise RuntimeError("scale must be positive")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype != dtype or _rows(out, copy=False) is None:
-        raise RuntimeError("out must be shaped like q, of its type, heads on 16-byte boundaries with unit stride")
+        op, o0, o1 = out.data_ptr(), heads * dim, dim
+    else:
+        got = _rows(out, copy=False) if out.shape == shape and out.dtype == dtype else None
+        if got is None:
+            raise RuntimeError("out must be shaped like q, of its type, heads on 16-byte boundaries with unit stride")
+        _, op, o0, o1 = got
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if rows:
         q, qp, q0, q1 = _rows(q)
-        _, op, o0, o1 = _rows(out, copy=False)
         n = _scratch_size(R, heads, kv_heads, dim)
         # the scratch is the call's own (a captured graph keeps its own, too)
         scratch = q.new_empty(n, dtype=torch.uint8)
