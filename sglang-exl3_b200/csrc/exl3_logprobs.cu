@@ -18,7 +18,7 @@
 // equal logits come in the order of their ids.
 //
 // Bound by HBM where rows are many: 2048 x 128256 bf16 (525 MB) take 92 us, 5.7 TB/s; what is
-// left is the exponential (16 a clock and SM, 60 us of it here) beside five other
+// left is the exponential (16 a clock and SM, 60 us of it here) beside nearly seven other
 // instructions an element.  Whole rows to a CTA beat equal runs of units over all rows joined
 // by a second kernel (107 us; 500 x 151936 fp32: 57 instead of 77 us): a row's finish costs
 // more than an uneven last wave.  Few rows are a chain of latencies: 1 x 128256 9 us, 80 x

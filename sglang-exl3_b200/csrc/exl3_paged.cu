@@ -272,7 +272,7 @@ struct AttnArgs {
     long long c_page, c_pos, c_head;             // bytes
     long long table_row;
     int seqs, rows, group, kv_heads, mblocks, mrows, mtotal;  // rows per sequence; m = row * group + head of the group
-    int max_pages, page_size, num_pages, capacity;
+    int page_size, num_pages, capacity;
     unsigned page_mul;
     int page_sh1, page_sh2;
     int window;
@@ -413,7 +413,7 @@ template <int UNIT> struct Walk {
 __device__ __forceinline__ int attn_length(const AttnArgs& a, int s) { return min(max(__ldg(a.lens + s), 0), a.capacity); }
 
 // One CTA: its run of units, warp w the positions w * kPos .. of each, through a ring of
-// stages of its own (no barrier but at an item's end).  The cache is the MMAs' A operand and
+// stages of its own (no barrier within an item).  The cache is the MMAs' A operand and
 // the query rows (heads of the group, rows of the sequence) their N, so that 8 heads fill an
 // MMA without padding: S^T = K Q^T, its columns' running maxima and sums, the weights
 // transposed in registers (movmatrix) and O^T = V^T P^T.  (The query rows as the MMA's M,
@@ -1243,7 +1243,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     a.q_row = p->q_stride, a.q_head = p->q_head_stride, a.out_row = p->out_stride, a.out_head = p->out_head_stride;
     a.seqs = p->seqs, a.rows = p->rows_per_seq, a.group = p->q_heads / c.kv_heads, a.kv_heads = c.kv_heads;
     a.mblocks = sp.mblocks, a.mrows = sp.mrows, a.mtotal = sp.mtotal;
-    a.max_pages = p->max_pages, a.page_size = c.page_size, a.num_pages = c.pages, a.capacity = (int) capacity;
+    a.page_size = c.page_size, a.num_pages = c.pages, a.capacity = (int) capacity;
     // position / page_size as a multiplication (32-bit unsigned division by an invariant)
     int l = 0;
     while (l < 31 && (1u << l) < (unsigned) c.page_size) ++l;
