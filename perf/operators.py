@@ -12,7 +12,6 @@ With ``own`` false ``run`` computes them in elementary torch operations, with ``
 through the package.  ``exact`` restates the definitions in 64 bits.
 """
 
-import functools
 import math
 import os
 import random
@@ -27,7 +26,6 @@ _BYTES = {"bf16": 2, "fp16": 2, "fp32": 4, "e4m3": 1}
 _E4M3_MAX = 448.0
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sglang-exl3_b200")
     if root not in sys.path:
