@@ -323,7 +323,9 @@ __device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t&
         : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // weights as 16-bit hi + lo pairs: together about twice the type's significant bits, so
-// that rounding the weights costs nothing beside the rounding of the output
+// that rounding the weights costs nothing beside the rounding of the output (single fp16
+// weights for e4m3 caches under bf16 queries: verify 57.5 us instead of 61.7, but 9 % of its
+// outputs a step of bf16 away from the rounded definition; pairs: 0.05 %)
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, __nv_bfloat16)
 {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -423,22 +425,20 @@ __device__ __forceinline__ int attn_length(const AttnArgs& a, int s) { return mi
 // copies three stages deep; pages are looked up a stage ahead.  Bound by HBM where the cache
 // is large: 64 sequences of up to 16384 (2.69 GB, bf16, 64 / 8 heads of 128) take 397 us with
 // the join, 6.8 TB/s.  With e4m3 caches or 64-wide heads half the bytes carry the same
-// instructions: 16 x 16384 e4m3, 32 / 4 heads, 52 us, 5.2 TB/s.  40 query rows (5 rows of 8
-// heads) hold 160 accumulators a thread: two warps a scheduler, issue-bound at 2.4 TB/s
-// (111 us; as two items of 20 rows, the cache read twice: 114 us).  Small batches are a
-// chain of latencies: 1 x 2049, 64 / 8 heads, 12 us in two kernels.
+// instructions: 16 x 16384 e4m3, 32 / 4 heads, 53 us, 5.1 TB/s.  40 query rows (5 rows of 8
+// heads) hold 160 accumulators a thread: 255 registers (of which 100 bytes spill), two warps
+// a scheduler and nothing to hide their latencies with, 1.95 TB/s (137 us; as two items of
+// 20 rows, the cache read twice, the same 137 us, but 176 instead of 141 over a bf16 cache).
+// Small batches are a chain of latencies: 1 x 2049, 64 / 8 heads, 12 us in two kernels.
 template <int D, typename QT, bool F8, int NT>
 __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using S = AttnShape<D, F8>;
     using MT = typename std::conditional<F8, __half, QT>::type;      // the MMAs' type
     constexpr float kRef = weight_ref<MT>();
-    // An e4m3 cache with bf16 queries takes the weights as one fp16 each, off by 2^-11 at most
-    // beside the 2^-8 of the output's rounding; the others as hi + lo pairs.
-    constexpr bool kLo = !(F8 && std::is_same<QT, __nv_bfloat16>::value);
     constexpr bool kRowScale = F8 && !std::is_same<QT, __half>::value;  // bf16 queries taken into fp16's range row by row
     constexpr bool kQShared = NT > 2;
-    constexpr int kBlocks = S::kPos == 32 && NT <= 3 ? 2 : 1;  // 16-position blocks of a step (e4m3, 24 rows: 78.5 -> 68.5 us for 16 x 16384)
+    constexpr int kBlocks = S::kPos == 32 && NT <= 3 ? 2 : 1;  // 16-position blocks of a step (e4m3, 24 rows: 92.9 -> 78.2 us for 16 x 16384)
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float sh_m[kAttnWarps][8 * NT], sh_l[kAttnWarps][8 * NT];
     __shared__ int sh_start[3], sh_len[32 * kAttnWarps];
@@ -817,7 +817,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                 }
             }
             // weights, as B fragments (rows x positions)
-            uint32_t hi[kBlocks][NT][2], lo[kBlocks][NT][kLo ? 2 : 1];
+            uint32_t hi[kBlocks][NT][2], lo[kBlocks][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float2 t = factor(nt);
@@ -829,13 +829,9 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                     const float x = ex2(fmaf(s[b][nt][2 * hf], t.x, f0)), y = ex2(fmaf(s[b][nt][2 * hf + 1], t.y, f1));
                     rl[nt][0] += x;
                     rl[nt][1] += y;
-                    if constexpr (kLo) {
-                        split2(x, y, hi[b][nt][hf], lo[b][nt][hf], MT());
-                        lo[b][nt][hf] = pg_transpose(lo[b][nt][hf]);
-                    } else {
-                        hi[b][nt][hf] = pack2(x, y, MT());
-                    }
+                    split2(x, y, hi[b][nt][hf], lo[b][nt][hf], MT());
                     hi[b][nt][hf] = pg_transpose(hi[b][nt][hf]);
+                    lo[b][nt][hf] = pg_transpose(lo[b][nt][hf]);
                 }
             }
             if constexpr (F8) {
@@ -854,7 +850,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, hi[b][nt][0], hi[b][nt][1]);
 #pragma unroll
-                        for (int nt = 0; kLo && nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[b][nt][0], lo[b][nt][kLo]);
+                        for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j + i][nt], v, lo[b][nt][0], lo[b][nt][1]);
                     }
                 }
             } else {
@@ -867,7 +863,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, hi[b][nt][0], hi[b][nt][1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[b][nt][0], lo[b][nt][kLo]);
+                    for (int nt = 0; nt < NT; ++nt) mma16816<MT>(o[j][nt], v, lo[b][nt][0], lo[b][nt][1]);
                 }
             }
         }

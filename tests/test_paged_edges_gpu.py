@@ -1,0 +1,37 @@
+"""Paged-cache operators at the edges of what their documentation allows, against the definitions
+of test_paged_gpu (whose tolerances hold here, except where a test derives its own)."""
+
+import pytest
+import torch
+
+from exl3_b200 import ops, paged
+from test_paged_gpu import BF16, E4M3, attention_oracle, build, half_step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("lens,heads,hk,dim,R,cap", [
+    ([1000, 129, 40, 2], 16, 2, 128, 1, 0.0),
+    ([2000, 513], 32, 4, 128, 5, 0.0),
+    ([1500, 31], 24, 1, 64, 1, 0.0),
+    ([700, 90], 8, 2, 64, 2, 20.0),
+])
+def test_e4m3_weights_keep_their_bits(cuda_device, lens, heads, hk, dim, R, cap):
+    """An e4m3 cache under bf16 queries carries its softmax weights as exactly as the other types:
+    before its rounding an output is off by (2 delta + 2^-15) max|v| at most, delta the scores'
+    error.  What is typical: with values of random signs an output and its error are both sums of
+    w_i v_i, the error's terms times a weight's relative error, so that e is about that error times
+    |o|.  bf16's spacing is at least 2^-8 |o|; an error e rounds to another value with a chance of
+    e / spacing.  Pairs of fp16 (2^-22) with fp32 scores of order 1 (2^-21 from 128 products) and
+    fp32 sums make e about 2^-20 |o|, a share of 2^-12 of the outputs; single fp16 weights (an rms of
+    2^-12.3) make it 2^-4.3 = 1/20.  The test draws the line between the two, at 1/64."""
+    q, k, v, table, n, (ks, vs) = build(lens, heads, hk, dim, BF16, E4M3, 16, R, cuda_device, seed=dim + R)
+    q = (q.float() / 8).to(BF16)  # scores of order 1: many weights take part
+    ref, rlse, vmax, smax = attention_oracle(q, k, v, table, lens, R, dim ** -0.5, cap, 0, ks, vs)
+    out = paged.attention(q, k, v, table, n, rows_per_seq=R, softcap=cap, k_scale=ks, v_scale=vs)
+    delta = dim * 2.0 ** -24 * smax
+    err = (out.double().cpu() - ref).abs()
+    assert (err <= (2 * delta + 2.0 ** -15) * vmax + half_step(BF16) * ref.abs()).all()
+    flips = (out.cpu() != ref.to(BF16)).double().mean()
+    assert float(flips) < 1 / 64, float(flips)
+    assert ops.device_status(cuda_device) == 0
