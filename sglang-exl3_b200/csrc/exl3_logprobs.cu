@@ -121,6 +121,10 @@ __device__ __forceinline__ float lp_low(float x)
     asm("max.NaN.f32 %0, %1, 0fF149F2CA;" : "=f"(r) : "f"(x));  // -1e30
     return r;
 }
+// A thread's first reference (base 2): so far above what -inf is lifted to that a lifted
+// element's exponent gives 0 (fp16: -65504 log2 e = -94502.3, 502 below), and below every
+// logit that counts - where a row's maximum is itself that far down lp_far holds.
+template <typename T> __device__ __forceinline__ constexpr float lp_start() { return std::is_same<T, __half>::value ? -9.4e4f : -1e30f; }
 template <typename T> __device__ __forceinline__ float2 lp_float2(uint32_t w)
 {
     if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
     const LpRow<T> r(a, row);
     const int nv = r.vectors();
     const int v0 = c0 * kLpThreads + tid, v1 = min(nv, c1 * kLpThreads);  // vectors v0, v0 + 256, ... of this thread
-    float best = -INFINITY, second = -INFINITY, ref = -1e30f;
+    float best = -INFINITY, second = -INFINITY, ref = lp_start<T>();
     f32x2 s2 = lp_pair(0.f, 0.f), t2 = s2;
     int bv = v0;
     // vectors b .. b + n of the row into L2, one request of one thread
