@@ -1,11 +1,14 @@
 // Log-probabilities of given tokens, the distribution's entropy and its top alternatives, in
 // one pass over the logits (exl3b200_token_logprobs).
 //
-//   lse = M + log sum_i exp(x_i - M)     logprob(t) = x_t - lse
+//   lse = M + log sum_i exp(x_i - M)     logprob(t) = (x_t - M) - log S
 //   H   = lse - sum_i p_i x_i            = log S - T / S   with y_i = x_i - M,
 //                                          S = sum exp(y_i), T = sum y_i exp(y_i)
 //
-// in base 2 throughout (y = x log2(e) - M2).  A row of 16-bit or fp32 logits is cut into
+// the sums in base 2.  M is subtracted before anything is rounded - x log2(e) less a reference
+// is one fused multiply-add, as is the reference less M log2(e) by which the sums are rescaled
+// to M itself - so that logits with a large common offset lose no accuracy (rounding M log2(e)
+// on one side alone cost 9e-5 at logits around 3000).  A row of 16-bit or fp32 logits is cut into
 // units of 256 vectors of 8 elements and is one CTA's, or - when rows are few - a cluster's
 // of up to 8 CTAs, whose first joins the pieces through distributed shared memory in a fixed
 // order.
@@ -245,21 +248,20 @@ template <typename T> struct LpRow {
     __device__ __forceinline__ int vectors() const { return (end + kLpVec - 1) / kLpVec; }
 };
 
-// A finite logit for which (x - M) is taken instead of x log2 e - M2: its product might
-// overflow, or it is near the bound to which the main loop lifts -inf (so that y e is 0 and
-// not NaN): -1e30, in fp16 the lowest value.
+// A row's finite maximum for which the sums are taken again from (x - M): its product with
+// log2 e might overflow, or it is near the bound to which the main loop lifts -inf (so that
+// y e is 0 and not NaN): -1e30, in fp16 the lowest value.
 template <typename T> __device__ __forceinline__ bool lp_far(float M)
 {
     return (fabsf(M) > 1e29f && fabsf(M) < INFINITY) || (std::is_same<T, __half>::value && M < -3e4f && M > -INFINITY);
 }
 
-// A row's results from its maximum M, S and T (relative to M2 = M log2 e) and warp 0's
-// descending keys.
+// A row's results from its maximum M, S and T (relative to M) and warp 0's descending keys.
 template <typename T>
 __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, float M, float S, float Tt, u64 key, int tid)
 {
-    const float M2 = M * kLpLog2e, ls = log2f(S);
-    auto of = [&](float x) { return lp_far<T>(M) || lp_far<T>(x) ? (x - M) - ls * kLpLn2 : (fmaf(x, kLpLog2e, -M2) - ls) * kLpLn2; };
+    const float ls = log2f(S);
+    auto of = [&](float x) { return fmaf(-ls, kLpLn2, x - M); };
     if (tid == 0) {
         const long long t = a.tokens[row];
         float lp = -INFINITY;  // an id outside the vocabulary has no probability
@@ -288,7 +290,7 @@ __device__ __forceinline__ void lp_join(const LogprobArgs& a, int row, int piece
         for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
         for (int p = lane; p < pieces; p += 32) {
             const float4 q = part(p);
-            const float d = lp_far<T>(M) ? (q.x - M) * kLpLog2e : q.x * kLpLog2e - M * kLpLog2e, k = lp_ex2(d);
+            const float d = (q.x - M) * kLpLog2e, k = lp_ex2(d);
             S += q.y * k;
             Tt += k == 0.f ? 0.f : (q.z + d * q.y) * k;
         }
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void exl3_logprobs_kernel(const __gr
             }
         }
     } else {
-        const float d = ref - M * kLpLog2e, k = s == 0.f ? 0.f : lp_ex2(d);
+        const float d = fmaf(-M, kLpLog2e, ref), k = s == 0.f ? 0.f : lp_ex2(d);
         t = s == 0.f ? 0.f : (t + d * s) * k;
         s *= k;
     }

@@ -111,3 +111,17 @@ def test_fp16_row_of_excluded_tokens_alone(cuda_device):
     assert torch.isnan(got.logprob[1]) and torch.isnan(got.entropy[1]) and torch.isnan(got.top_logprobs[1]).all()
     assert torch.equal(got.top_ids.cpu(), torch.arange(4).expand(3, 4))
     assert (got.logprob[::2] + math.log(30000)).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("rows", [5, 600])
+@pytest.mark.parametrize("offset,dtype", [(0, torch.float32), (300, torch.float32), (3000, torch.float32), (-3000, torch.float32),
+                                          (30000, torch.float32), (1e6, torch.float32), (300, torch.bfloat16), (300, torch.float16),
+                                          (-2000, torch.float16)])
+def test_a_common_offset_costs_no_accuracy(cuda_device, offset, dtype, rows):
+    n = 20001
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(3)
+    x = (torch.randn(rows, n, generator=g, device=cuda_device) * 3 + offset).to(dtype)
+    tokens = torch.randint(0, n, (rows,), generator=g, device=cuda_device)
+    tokens[::2] = x[::2].argmax(-1)
+    check(x, tokens, 5, LP.token_logprobs(x, tokens, 5))
