@@ -274,12 +274,22 @@ class VerifyModel:
         """The verify step's verdict on the draft: for every row but a sequence's last, the
         log-probability that the model gives the next drafted token (``self.tokens[:, j + 1]``),
         its entropy there and the ``top`` tokens it would rather have; the last row has no drafted
-        token (-inf).  Shaped like the rows, ``[batch * rows_per_seq]``, from the step's logits."""
+        token (-inf).  Shaped like the rows, ``[batch * rows_per_seq]``, from the step's logits.
+        On the current stream: after the steps replayed so far, and before the next."""
         if self.logits is None:
             raise RuntimeError("run a verify step first")
+        # replay() runs on self.stream; a call that is being captured has no such wait to record,
+        # its replays come after the step by the caller's order
+        cur = torch.cuda.current_stream(self.device)
+        apart = cur != self.stream and not torch.cuda.is_current_stream_capturing()
+        if apart:
+            cur.wait_stream(self.stream)
         want = torch.full_like(self.tokens, -1)
         want[:, :-1] = self.tokens[:, 1:]
-        return token_logprobs(self.logits, want.view(-1), top)
+        got = token_logprobs(self.logits, want.view(-1), top)
+        if apart:
+            self.stream.wait_stream(cur)
+        return got
 
     def replay(self, n: int = 1) -> None:
         with torch.cuda.stream(self.stream):

@@ -1,0 +1,53 @@
+"""The paged model and the verify model at the ends of their caches and between streams."""
+
+import dataclasses
+
+import pytest
+import torch
+
+from exl3_b200.verify import CONFIG5, VerifyModel
+
+pytestmark = pytest.mark.gpu
+
+
+def test_draft_logprobs_follow_the_replayed_step(cuda_device):
+    """replay() and draft_logprobs() one after the other without a wait between: the report is of the
+    step just replayed, and the step replayed next leaves it alone.  Tolerance: fp32 logits of size
+    S give log-probabilities off by far less than 1e-5 (1 + S)."""
+    cfg = dataclasses.replace(CONFIG5, layers=6, hidden=1024, heads=8, kv_heads=2, experts=16, inter=512, vocab=32000)
+    m = VerifyModel(cfg, 2, 64 + cfg.rows_per_seq, cuda_device)
+    m.fill_random_kv(64)
+    m.capture()
+    torch.cuda.synchronize()
+    drafts = [torch.randint(0, cfg.vocab, m.tokens.shape, generator=torch.Generator().manual_seed(k)).to(cuda_device)
+              for k in range(4)]
+    reports, snaps = [], []
+    for k, draft in enumerate(drafts):
+        with torch.cuda.stream(m.stream):
+            m.tokens.copy_(draft)
+        m.replay(3)
+        reports.append(m.draft_logprobs(top=2))
+        with torch.cuda.stream(m.stream):  # the logits that the report is of, as the stream has them
+            snaps.append(m.logits.clone())
+    torch.cuda.synchronize()
+    for draft, got, logits in zip(drafts, reports, snaps):
+        ref = torch.log_softmax(logits.double(), -1).view(2, cfg.rows_per_seq, -1)
+        want = torch.gather(ref[:, :-1], 2, draft[:, 1:, None])[..., 0]
+        lp = got.logprob.view(2, cfg.rows_per_seq)
+        tol = 1e-5 * (1 + float(logits.abs().max()))
+        assert (lp[:, :-1].double() - want).abs().max() < tol and (lp[:, -1] == -float("inf")).all()
+        assert torch.equal(got.top_ids.view(2, cfg.rows_per_seq, 2)[..., 0], logits.argmax(-1).view(2, -1))
+    assert not torch.equal(reports[0].logprob, reports[1].logprob)
+    # on the model's own stream, and captured into a graph of the caller's
+    with torch.cuda.stream(m.stream):
+        own = m.draft_logprobs(top=2)
+    torch.cuda.synchronize()
+    assert torch.equal(own.logprob, reports[-1].logprob)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = m.draft_logprobs(top=2)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held.logprob, own.logprob) and torch.equal(held.top_ids, own.top_ids)
+    del g
+    m.close()
