@@ -310,10 +310,10 @@ class DecodeModel:
         pos0 = self.pos.clone()
         tok0 = self.tokens.clone()
         with torch.cuda.stream(s):
-            for _ in range(2):
+            for _ in range(2):  # each from where the sequences stand: the last free position serves both
                 self.step()
-            self.pos.copy_(pos0)
-            self.tokens.copy_(tok0)
+                self.pos.copy_(pos0)
+                self.tokens.copy_(tok0)
             torch.cuda.synchronize(self.device)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, stream=s):

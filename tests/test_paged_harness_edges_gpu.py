@@ -5,7 +5,9 @@ import dataclasses
 import pytest
 import torch
 
+from exl3_b200 import ops
 from exl3_b200.verify import CONFIG5, VerifyModel
+from test_paged_harness_gpu import _paged
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +53,23 @@ def test_draft_logprobs_follow_the_replayed_step(cuda_device):
     assert torch.equal(held.logprob, own.logprob) and torch.equal(held.top_ids, own.top_ids)
     del g
     m.close()
+
+
+def test_capture_with_one_position_left(cuda_device):
+    """Capturing warms up without leaving the pages: a sequence with a single position left is
+    captured and generates its last token."""
+    m = _paged(3, 64, cuda_device, page_size=16, logprobs=2)
+    m.fill_random_kv([63, 5, 40])
+    before = m.k_cache.clone()
+    m.tokens.copy_(torch.tensor([9, 8, 7]))
+    m.capture()
+    assert ops.device_status(cuda_device) == 0
+    assert m.pos.tolist() == [63, 5, 40] and m.tokens.tolist() == [9, 8, 7]
+    for b, n in enumerate([63, 5, 40]):  # what the sequences hold is as it was
+        for p in range(n):
+            page = int(m.block_table[b, p // 16])
+            assert torch.equal(m.k_cache[:, page, p % 16], before[:, page, p % 16])
+    tokens, lp = m.generate(torch.tensor([5, 6, 4]), 1)
+    assert tokens.shape == (3, 1) and torch.isfinite(lp.logprob).all() and m.pos.tolist() == [64, 6, 41]
+    assert ops.device_status(cuda_device) == 0
+    m.release()
