@@ -112,6 +112,7 @@ class DecodeModel:
         self.ln_f = torch.ones(H, dtype=torch.bfloat16, device=device)
         self.paged, self.page_size, self.n_logprobs = bool(paged), int(page_size), logprobs
         self.logprobs = None
+        self._graph_outputs = None  # the captured step's logits and log-probabilities
         if self.paged:
             # [layer][pages, page_size, kv_heads_local, head_dim]; a sequence's pages lie apart
             per_seq = -(-max_ctx // self.page_size)
@@ -322,6 +323,7 @@ class DecodeModel:
         self.pos.copy_(pos0)
         self.tokens.copy_(tok0)
         self.graph = g
+        self._graph_outputs = self.last_logits, self.logprobs
         self.stream = s
         return g
 
@@ -359,6 +361,7 @@ class DecodeModel:
         host_in.copy_(prompt_tokens.to(torch.long))
         L = _lib.lib()
         lps = None
+        self.last_logits, self.logprobs = self._graph_outputs  # (an eager step since the capture left its own)
         if self.n_logprobs is not None:
             lps = [None if t is None else torch.empty((self.batch, n) + t.shape[1:], dtype=t.dtype)
                    for t in self.logprobs]
@@ -392,6 +395,7 @@ class DecodeModel:
         """Run n captured decode steps (feeding back the greedy tokens)."""
         if self.graph is None:
             raise RuntimeError("call capture() first")
+        self.last_logits, self.logprobs = self._graph_outputs
         with torch.cuda.stream(self.stream):
             for _ in range(n):
                 self.graph.replay()

@@ -73,3 +73,24 @@ def test_capture_with_one_position_left(cuda_device):
     assert tokens.shape == (3, 1) and torch.isfinite(lp.logprob).all() and m.pos.tolist() == [64, 6, 41]
     assert ops.device_status(cuda_device) == 0
     m.release()
+
+
+def test_generate_reports_its_own_steps(cuda_device):
+    """A step outside the graph between capture() and generate() leaves generate's report its own:
+    of the tokens generated, from the logits of the captured step."""
+    m = _paged(2, 128, cuda_device, page_size=16, logprobs=3)
+    m.fill_random_kv([40, 9])
+    pos = m.pos.clone()
+    m.capture()
+    m.tokens.copy_(torch.tensor([700, 800]))
+    m.step()  # eager, of other tokens
+    eager = m.logprobs
+    m.pos.copy_(pos)
+    torch.cuda.synchronize()
+    tokens, lp = m.generate(torch.tensor([5, 6]), 4)
+    assert m.logprobs is not eager
+    assert torch.equal(lp.top_ids[..., 0], tokens)  # greedy (equal logits: the lower id first, as argmax)
+    last = torch.log_softmax(m.last_logits.double(), -1).cpu()
+    assert (lp.logprob[:, -1].double() - last.amax(-1)).abs().max() < 1e-5
+    assert all(len(set(row)) > 1 for row in lp.logprob.tolist())
+    m.release()
