@@ -573,8 +573,8 @@ typedef struct exl3b200_paged_cache {
  *
  * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] of in_dtype (F16,
  * BF16 or F32) with token and head strides in elements; q_out of q_out_dtype (F16 or BF16;
- * the cache's dtype unless that is E4M3); it may be q itself.  All bases and strides
- * multiples of 16 bytes.  rotary: a multiple of 16 up to head_dim (0: no rotation).
+ * the cache's dtype unless that is E4M3); it may be q itself, and its rows must not overlap
+ * one another (EXL3B200_EBADSHAPE).  All bases and strides multiples of 16 bytes.  rotary: a multiple of 16 up to head_dim (0: no rotation).
  * positions and slots: device int64 [tokens]; inv_freq device fp32 [rotary/2].  A negative
  * slot (a padding row) leaves the cache as it is; one past the pool does too and records
  * EXL3B200_EBADARG in the device status.  Slots of one call must differ.
@@ -612,7 +612,7 @@ EXL3B200_API int exl3b200_rope_append(const exl3b200_rope_append_args* args, voi
  *
  * q and out [seqs * rows_per_seq][q_heads][head_dim] of dtype F16 or BF16 (the cache's
  * unless that is E4M3), row and head strides in elements, multiples of 8, 16-byte aligned
- * bases.  block_table: device int32 [seqs][max_pages], row stride table_stride; seq_lens:
+ * bases; out's rows must not overlap one another (EXL3B200_EBADSHAPE).  block_table: device int32 [seqs][max_pages], row stride table_stride; seq_lens:
  * device int32 [seqs], the new tokens included.  A length over max_pages * page_size is cut
  * to it, a page id outside the pool reads as zeros; both record EXL3B200_EBADARG in the
  * device status.  A NaN or infinity in v at a position that one row of a sequence sees may

@@ -6,6 +6,8 @@
 // dimension is contiguous, 16 bit or e4m3 with one fp32 scale per kv head.
 #include <climits>
 #include <cmath>
+#include <cstdlib>
+#include <utility>
 
 #include <cuda_fp8.h>
 
@@ -1064,6 +1066,16 @@ static int paged_launch(Kern kern, dim3 grid, int block, int smem, cudaStream_t 
 
 static bool misaligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 
+// whether two of an output's n0 x n1 rows of d elements share an address (an expanded view):
+// several CTAs would write it
+static bool overlapping(long long n0, long long s0, long long n1, long long s1, int d)
+{
+    s0 = std::abs(s0), s1 = std::abs(s1);
+    if (n0 <= 1 || n1 <= 1) return (n0 > 1 && s0 < d) || (n1 > 1 && s1 < d);
+    if (s0 < s1) std::swap(s0, s1), std::swap(n0, n1);
+    return s1 < d || s0 < (n1 - 1) * s1 + d;
+}
+
 // the strides of a cache, in bytes; false: a row would not begin on a 16-byte boundary
 static bool cache_strides(const exl3b200_paged_cache& c, long long* page, long long* pos, long long* head)
 {
@@ -1178,6 +1190,7 @@ extern "C" int exl3b200_rope_append(const exl3b200_rope_append_args* p, void* st
         if (s % vec) return kErrUnaligned;
     if (p->q_out_stride % 8 || p->q_out_head_stride % 8) return kErrUnaligned;
     if (misaligned(p->q, 16) || misaligned(p->k, 16) || misaligned(p->v, 16) || misaligned(p->q_out, 16)) return kErrUnaligned;
+    if (overlapping(p->tokens, p->q_out_stride, p->q_heads, p->q_out_head_stride, c.head_dim)) return kErrBadShape;
     AppendArgs a = {};
     if (!cache_strides(c, &a.c_page, &a.c_pos, &a.c_head)) return kErrUnaligned;
     a.q = p->q, a.k = p->k, a.v = p->v, a.q_out = p->q_out;
@@ -1220,6 +1233,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     if (scratch_bytes < need) return kErrWorkspace;
     if (misaligned(scratch, 256) || misaligned(p->q, 16) || misaligned(p->out, 16)) return kErrUnaligned;
     if (p->q_stride % 8 || p->q_head_stride % 8 || p->out_stride % 8 || p->out_head_stride % 8) return kErrUnaligned;
+    if (overlapping((long long) p->seqs * p->rows_per_seq, p->out_stride, p->q_heads, p->out_head_stride, c.head_dim)) return kErrBadShape;
     AttnArgs a = {};
     if (!cache_strides(c, &a.c_page, &a.c_pos, &a.c_head)) return kErrUnaligned;
     const AttnSplit sp = attn_split(p->rows_per_seq, p->q_heads / c.kv_heads, c.head_dim);

@@ -103,7 +103,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     (2i, 2i + 1) with ``interleaved``.  ``positions`` and ``slots``: int64 ``[tokens]``; a
     negative slot writes nothing (padding rows), one past the pool neither, and is recorded
     in ``ops.device_status``.  The slots of one call must differ.  ``q_out`` (default: new,
-    in the cache's type, bf16 for an e4m3 cache) may be ``q``."""
+    in the cache's type, bf16 for an e4m3 cache) may be ``q``; an expanded view is refused."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     index = k_cache.get_device()
     if not (q.get_device() == k.get_device() == v.get_device() == positions.get_device() == slots.get_device()
@@ -164,7 +164,8 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     before its window, are not read), ``seq_lens`` int32 ``[sequences]``.  ``scale`` defaults
     to ``head_dim ** -0.5``; ``softcap`` > 0 caps scores at ``softcap * tanh(s / softcap)``.
     Rows that see nothing (an empty sequence) are zeros, their ``lse`` is -inf.  Returns
-    ``out`` (q's type), with ``return_lse`` also fp32 ``lse [rows, q_heads]``."""
+    ``out`` (q's type; a given one must not be an expanded view), with ``return_lse`` also
+    fp32 ``lse [rows, q_heads]``."""
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     index = k_cache.get_device()
     if not q.get_device() == block_table.get_device() == seq_lens.get_device() == index:

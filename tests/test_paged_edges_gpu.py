@@ -35,3 +35,22 @@ def test_e4m3_weights_keep_their_bits(cuda_device, lens, heads, hk, dim, R, cap)
     flips = (out.cpu() != ref.to(BF16)).double().mean()
     assert float(flips) < 1 / 64, float(flips)
     assert ops.device_status(cuda_device) == 0
+
+
+def test_expanded_outputs_are_refused(cuda_device):
+    """Several CTAs would write one address; inputs may be expanded."""
+    lens, heads, hk, dim = [20, 30], 4, 2, 64
+    q, k, v, table, n, _ = build(lens, heads, hk, dim, BF16, BF16, 16, 1, cuda_device)
+    slots = torch.tensor([-1, -1], device=cuda_device)
+    new = torch.zeros(1, hk, dim, dtype=BF16, device=cuda_device).expand(2, -1, -1)
+    inv = torch.ones(dim // 2, device=cuda_device)
+    for bad in (q[:1].expand(2, -1, -1), q[:, :1].expand(-1, heads, -1), q[:1, :1].expand(2, heads, -1)):
+        with pytest.raises(RuntimeError, match="EBADSHAPE"):
+            paged.attention(q, k, v, table, n, out=bad)
+        with pytest.raises(RuntimeError, match="EBADSHAPE"):
+            paged.rope_append(q, new, new, k, v, slots, slots, inv, q_out=bad)
+    one = q[:1].expand(2, -1, -1)
+    got = paged.attention(one, k, v, table, n)
+    assert torch.equal(got, paged.attention(one.contiguous(), k, v, table, n))
+    assert torch.equal(paged.rope_append(one, new, new, k, v, slots, slots, inv)[1],
+                       paged.rope_append(q[:1], new[:1], new[:1], k, v, slots[:1], slots[:1], inv)[0])
