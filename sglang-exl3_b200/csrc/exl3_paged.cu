@@ -4,6 +4,7 @@
 //
 // A cache is [pages][page_size][kv_heads][head_dim] in any stride order whose last
 // dimension is contiguous, 16 bit or e4m3 with one fp32 scale per kv head.
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdlib>
@@ -1118,13 +1119,13 @@ template <int D, typename QT, bool F8, int NT>
 static int attn_launch(const AttnArgs& a, int ctas, cudaStream_t st)
 {
     constexpr int smem = AttnShape<D, F8>::smem(NT);
-    static bool done[64] = {false};
+    static std::atomic<bool> done[64];  // threads that race on the first call set the same value
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kErrLaunch;
     auto kern = exl3_paged_attn_kernel<D, QT, F8, NT>;
-    if (!done[dev]) {
+    if (!done[dev].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrLaunch;
-        done[dev] = true;
+        done[dev].store(true, std::memory_order_release);
     }
     const int rc = paged_launch(kern, dim3((unsigned) ctas), 32 * kAttnWarps, smem, st, a);
     if (rc != kOk) return rc;

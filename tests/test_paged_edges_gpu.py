@@ -1,11 +1,13 @@
 """Paged-cache operators at the edges of what their documentation allows, against the definitions
 of test_paged_gpu (whose tolerances hold here, except where a test derives its own)."""
 
+import threading
+
 import pytest
 import torch
 
 from exl3_b200 import ops, paged
-from test_paged_gpu import BF16, E4M3, attention_oracle, build, half_step
+from test_paged_gpu import BF16, E4M3, FP16, attention_oracle, build, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +56,33 @@ def test_expanded_outputs_are_refused(cuda_device):
     assert torch.equal(got, paged.attention(one.contiguous(), k, v, table, n))
     assert torch.equal(paged.rope_append(one, new, new, k, v, slots, slots, inv)[1],
                        paged.rope_append(q[:1], new[:1], new[:1], k, v, slots[:1], slots[:1], inv)[0])
+
+
+def test_calls_from_several_threads(cuda_device):
+    """Threads that call at once, each on a stream of its own, the first call of every kernel among
+    them, get what a single thread gets."""
+    jobs = []
+    for heads, hk, dim, qt, ct in ((20, 1, 64, FP16, FP16), (8, 8, 64, BF16, E4M3), (18, 2, 128, FP16, E4M3), (34, 2, 128, FP16, FP16)):
+        q, k, v, table, n, (ks, vs) = build([300, 77, 1], heads, hk, dim, qt, ct, 16, 1, cuda_device)
+        jobs.append(dict(q=q, k_cache=k, v_cache=v, block_table=table, seq_lens=n, k_scale=ks, v_scale=vs))
+    torch.cuda.synchronize()
+    start, got, wrong = threading.Barrier(8), [None] * 8, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(20):
+                    got[i] = paged.attention(**jobs[i % 4])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # the main thread raises it
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    for i in range(8):
+        assert torch.equal(got[i], paged.attention(**jobs[i % 4])), i
