@@ -6,7 +6,8 @@ import threading
 import pytest
 import torch
 
-from exl3_b200 import ops, paged
+from exl3_b200 import decode, ops, paged
+from exl3_b200.harness import DecodeModel, DecoderConfig
 from test_paged_gpu import BF16, E4M3, FP16, attention_oracle, build, half_step
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,44 @@ def test_calls_from_several_threads(cuda_device):
     assert not wrong, wrong
     for i in range(8):
         assert torch.equal(got[i], paged.attention(**jobs[i % 4])), i
+
+
+def test_prompt_appended_to_a_dense_cache(cuda_device):
+    """A prompt goes through a paged view into the dense cache of the fused decode sub-layer, which is
+    called right behind it: it attends to the new rows.  (The sub-layer requests rows of earlier
+    positions before its dependency wait.)  Against the same calls with a wait between; the matmuls'
+    sums may add in another order, so the residual streams agree to 1e-3, and to no such thing
+    with the cache as it was before."""
+    dev, ctx, hk = cuda_device, 700, 2
+    cfg = DecoderConfig(layers=1, hidden=512, heads=16, kv_heads=hk, head_dim=128, inter=1024, vocab=1024, K=4, cb=0)
+    m = DecodeModel(cfg, batch=1, max_ctx=1024, device=dev, fused=True)
+    for lin in m.layers[0]["qkv"] + [m.layers[0]["o"]]:
+        lin[2].mul_(float(lin[0].size(0) * 16) ** -0.5)
+    kc, vc = m.k_cache[0], m.v_cache[0]  # [1, hk, 1024, 128]
+    pages = [t.permute(0, 2, 1, 3) for t in (kc, vc)]
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(8)
+    q, k, v = (torch.randn(ctx, n, 128, generator=gen, device=dev).to(BF16) for n in (16, hk, hk))
+    at = torch.arange(ctx, device=dev)
+    pos = torch.full((), ctx, device=dev)
+    h0 = torch.randn(1, 512, generator=gen, device=dev)
+    L = m.layers[0]
+
+    def run(wait, append=True):
+        kc.zero_(), vc.fill_(3.0)
+        h, ss = h0.clone(), torch.zeros(2, 1, device=dev)
+        torch.sum(h * h, dim=-1, out=ss[0])
+        torch.cuda.synchronize()
+        if append:
+            paged.rope_append(q, k, v, *pages, at, at, m.inv_freq)
+        if wait:
+            torch.cuda.synchronize()
+        decode.decode_attention(h, ss[0], ss[1], L["ln1"], cfg.eps, L["qkv"], L["o"], cfg.K, cfg.cb, kc, vc, pos, m.inv_freq)
+        return h
+
+    want, before = run(True), run(True, append=False)
+    rel = lambda a, b: float((a - b).norm() / b.norm())  # noqa: E731
+    assert rel(before, want) > 1e-2
+    for _ in range(20):
+        assert rel(run(False), want) < 1e-3
+    assert ops.device_status(dev) == 0
