@@ -5,6 +5,7 @@
 // A cache is [pages][page_size][kv_heads][head_dim] in any stride order whose last
 // dimension is contiguous, 16 bit or e4m3 with one fp32 scale per kv head.
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdlib>
@@ -374,6 +375,9 @@ __device__ __forceinline__ float rcp(float x)
 // fp16 weights reach 2^14 so that small ones keep their bits: what is lost of a weight is
 // under 2^-31 of the largest.
 constexpr float kSlack = 8.f;
+// a positive factor of the scores, kept from 0, with which a masked -inf would become NaN, and from
+// infinity, with which a score of 0 would (a NaN stays one)
+__device__ __forceinline__ float in_range(float x) { return x < FLT_MIN ? FLT_MIN : x > FLT_MAX ? FLT_MAX : x; }
 constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing (finite: no case of its own in the loop)
 template <typename MT> __host__ __device__ constexpr float weight_ref() { return std::is_same<MT, __half>::value ? 6.f : 0.f; }
 
@@ -592,7 +596,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
             const int kvh = w.h / a.mblocks, mb = w.h - kvh * a.mblocks;
             mbase = mb * a.mrows;
             mcount = min(a.mrows, a.mtotal - mbase);
-            ks = ((F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale) * kLog2e;
+            ks = in_range(((F8 && a.k_scale) ? a.scale * __ldg(a.k_scale + kvh) : a.scale) * kLog2e);
             if (tid < 8 * NT) {  // (rows past the item's last repeat it and are not written)
                 const int mm = mbase + min(tid, mcount - 1), j = mm / a.group;
                 const int row = w.s * a.rows + j, head = kvh * a.group + mm - j * a.group;
@@ -639,7 +643,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                             amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
                             float down;
                             const float up = power(amax, &down);
-                            if (warp == 0 && c == 0) sh_rs[8 * nt + g] = ks * up;
+                            if (warp == 0 && c == 0) sh_rs[8 * nt + g] = in_range(ks * up);
 #pragma unroll
                             for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(32 * kAttnWarps, 2) void exl3_paged_attn_kernel(con
                         up = power(amax, &down);
                     }
                     if (m >= 8 * NT) continue;
-                    if (kRowScale && l8 == 0) sh_rs[m] = ks * up;
+                    if (kRowScale && l8 == 0) sh_rs[m] = in_range(ks * up);
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) {
                         const uint32_t x = kRowScale ? pack2(lo16(t[k][i]) * down, hi16(t[k][i]) * down, __half()) : t[k][i];

@@ -1,6 +1,7 @@
 """Paged-cache operators at the edges of what their documentation allows, against the definitions
 of test_paged_gpu (whose tolerances hold here, except where a test derives its own)."""
 
+import math
 import threading
 
 import pytest
@@ -128,3 +129,24 @@ def test_prompt_appended_to_a_dense_cache(cuda_device):
     for _ in range(20):
         assert rel(run(False), want) < 1e-3
     assert ops.device_status(dev) == 0
+
+
+@pytest.mark.parametrize("scale,qscale", [(2.0 ** -100, 2.0 ** -60), (2.0 ** -120, 2.0 ** -40), (2.0 ** -126, 1.0),
+                                          (2.0 ** 100, 2.0 ** 60)])
+def test_scores_that_vanish_leave_the_mean(cuda_device, scale, qscale):
+    """A scale and queries whose product leaves fp32's range, and scores that are 0 all the same (above
+    it: with keys of 0): the answer is the mean of the values, masked positions (the last stage's, a
+    later row's) as ever without weight."""
+    lens, heads, hk, dim, R = [3, 130, 0], 8, 2, 128, 2
+    for ct in (BF16, E4M3):
+        q, k, v, table, n, (ks, vs) = build(lens, heads, hk, dim, BF16, ct, 16, R, cuda_device)
+        q = (q.float() * qscale).to(BF16)
+        if qscale > 1:
+            k.view(torch.uint8).zero_()
+        ref, rlse, vmax, _ = attention_oracle(q, k, v, table, lens, R, scale, 0.0, 0, ks, vs)
+        out, lse = paged.attention(q, k, v, table, n, rows_per_seq=R, scale=scale, k_scale=ks, v_scale=vs, return_lse=True)
+        err = (out.double().cpu() - ref).abs()
+        assert (err <= 2.0 ** -15 * vmax + half_step(BF16) * ref.abs()).all()
+        empty = rlse == -math.inf
+        assert torch.equal(lse.cpu() == -math.inf, empty)
+        assert ((lse.double().cpu() - rlse)[~empty].abs() <= 2.0 ** -20 * (1 + rlse[~empty].abs())).all()
