@@ -613,8 +613,8 @@ EXL3B200_API int exl3b200_rope_append(const exl3b200_rope_append_args* args, voi
  * q and out [seqs * rows_per_seq][q_heads][head_dim] of dtype F16 or BF16 (the cache's
  * unless that is E4M3), row and head strides in elements, multiples of 8, 16-byte aligned
  * bases; out's rows must not overlap one another (EXL3B200_EBADSHAPE).  block_table: device int32 [seqs][max_pages], row stride table_stride; seq_lens:
- * device int32 [seqs], the new tokens included.  A length over max_pages * page_size is cut
- * to it, a page id outside the pool reads as zeros; both record EXL3B200_EBADARG in the
+ * device int32 [seqs], the new tokens included.  A length over max_pages * page_size (or over
+ * 2^31 - 2049) is cut to it, a page id outside the pool reads as zeros; both record EXL3B200_EBADARG in the
  * device status.  A NaN or infinity in v at a position that one row of a sequence sees may
  * reach the sequence's other rows; beyond that nothing behind a mask is read.
  *

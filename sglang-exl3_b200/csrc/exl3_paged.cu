@@ -1246,8 +1246,9 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     AttnArgs a = {};
     if (!cache_strides(c, &a.c_page, &a.c_pos, &a.c_head)) return kErrUnaligned;
     const AttnSplit sp = attn_split(p->rows_per_seq, p->q_heads / c.kv_heads, c.head_dim);
-    // positions are 32-bit, and so is the number of units of a launch
-    const long long capacity = std::min((long long) p->max_pages * c.page_size, (long long) INT_MAX - 256);
+    // positions are 32-bit, a length less the rows and a window and one rounded up to units among
+    // them, and so is the number of units of a launch
+    const long long capacity = std::min((long long) p->max_pages * c.page_size, (long long) INT_MAX - 2 * EXL3B200_PAGED_MAX_ROWS);
     if (((capacity + 63) / 64 + 1) * p->seqs * c.kv_heads * sp.mblocks > INT_MAX ||
         (long long) p->seqs * p->rows_per_seq * p->q_heads > INT_MAX)
         return kErrBadShape;

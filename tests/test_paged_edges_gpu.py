@@ -150,3 +150,19 @@ def test_scores_that_vanish_leave_the_mean(cuda_device, scale, qscale):
         empty = rlse == -math.inf
         assert torch.equal(lse.cpu() == -math.inf, empty)
         assert ((lse.double().cpu() - rlse)[~empty].abs() <= 2.0 ** -20 * (1 + rlse[~empty].abs())).all()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 257, 2 ** 31 - 258, 2 ** 31 - 2049, 2 ** 31 - 2050, 2 ** 31 - 1])
+def test_windows_near_two_to_the_31(cuda_device, window):
+    """Positions that a table of 2^31 could hold, a window of nearly as many, and sequences far shorter
+    than their rows: the window takes nothing away."""
+    page, R, dim, lens = 2 ** 20, 400, 64, [10, 450]
+    k, v = (torch.randn(1, page, 1, dim, device=cuda_device).to(BF16) for _ in range(2))
+    table = torch.zeros(2, 2048, dtype=torch.int32, device=cuda_device)
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    q = torch.randn(2 * R, 1, dim, device=cuda_device).to(BF16)
+    out, lse = paged.attention(q, k, v, table, n, rows_per_seq=R, window=window, return_lse=True)
+    small, sl = paged.attention(q, k, v, table[:, :1].contiguous(), n, rows_per_seq=R, return_lse=True)
+    assert torch.equal(out, small) and torch.equal(lse, sl)
+    assert torch.equal(torch.isinf(lse[:, 0]).cpu(), torch.arange(2 * R) < R - lens[0])
+    assert ops.device_status(cuda_device) == 0
