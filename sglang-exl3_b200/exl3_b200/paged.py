@@ -85,8 +85,12 @@ def _rows(t: torch.Tensor, copy: bool = True):
     copy), its address and its row and head strides; None where it is not and may not be copied."""
     s0, s1, s2 = t.stride()
     p = t.data_ptr()
-    if s2 != 1 or (s0 | s1) % (4 if t.dtype == torch.float32 else 8) or p % 16:
-        return _rows(t.clone(memory_format=torch.contiguous_format), False) if copy else None
+    vec = 4 if t.dtype == torch.float32 else 8
+    if s2 != 1 or (s0 | s1) % vec or p % 16:
+        # (the stride of a dimension of one does not count)
+        s0, s1 = s0 if t.size(0) > 1 else 0, s1 if t.size(1) > 1 else 0
+        if s2 != 1 or (s0 | s1) % vec or p % 16:
+            return _rows(t.clone(memory_format=torch.contiguous_format), False) if copy else None
     return t, p, s0, s1
 
 

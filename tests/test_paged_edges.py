@@ -36,3 +36,22 @@ def test_outputs_apart_are_taken(call, kw):
     if torch.cuda.is_available():
         pytest.skip("the addresses are not real ones")
     assert call(**kw) == _lib.ELAUNCH
+
+
+def test_rows_of_one_token_or_one_head():
+    """The stride of a dimension of one does not decide whether rows are aligned (a helper of the
+    wrappers; no device needed)."""
+    import torch
+
+    from exl3_b200 import paged
+
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    for shape, strides, ok in (((1, 4, 64), (259, 64, 1), True), ((3, 1, 64), (256, 67, 1), True), ((1, 1, 64), (3, 5, 1), True),
+                               ((2, 4, 64), (259, 64, 1), False), ((3, 2, 64), (256, 67, 1), False), ((1, 4, 64), (256, 60, 1), False)):
+        t = base.as_strided(shape, strides)
+        got = paged._rows(t, copy=False)
+        assert (got is not None) == ok
+        if ok:
+            assert got[0] is t and got[2] % 8 == 0 and got[3] % 8 == 0
+        copied = paged._rows(t)
+        assert (copied[0] is t) == ok and copied[2] % 8 == 0 and copied[3] % 8 == 0

@@ -166,3 +166,28 @@ def test_windows_near_two_to_the_31(cuda_device, window):
     assert torch.equal(out, small) and torch.equal(lse, sl)
     assert torch.equal(torch.isinf(lse[:, 0]).cpu(), torch.arange(2 * R) < R - lens[0])
     assert ops.device_status(cuda_device) == 0
+
+
+def test_strides_of_single_rows_do_not_count(cuda_device):
+    """One token, or one head, in a buffer of an odd width: its rows begin on 16-byte boundaries all the
+    same, and outputs there are written in place."""
+    for tokens, heads in ((1, 4), (3, 1)):
+        q, k, v, table, n, _ = build([40] * tokens, heads, 1, 64, BF16, BF16, 16, 1, cuda_device)
+        want = paged.attention(q, k, v, table, n)
+        if tokens == 1:
+            room = torch.zeros(2, heads * 64 + 3, dtype=BF16, device=cuda_device)
+            out, src = (t[:, :heads * 64].view(2, heads, 64)[:1] for t in (room, room + 0))
+        else:
+            room = torch.zeros(tokens, 67, 64, dtype=BF16, device=cuda_device)
+            out, src = (t.as_strided((tokens, 1, 64), (67 * 64, 67, 1)) for t in (room, room + 0))
+        src.copy_(q)
+        assert (out.stride(0) | out.stride(1)) % 8
+        got = paged.attention(src, k, v, table, n, out=out)
+        assert got.data_ptr() == room.data_ptr() and torch.equal(out, want)
+        slots = torch.full((tokens,), -1, device=cuda_device)
+        inv = torch.ones(32, device=cuda_device)
+        kv = torch.zeros(tokens, 1, 64, dtype=BF16, device=cuda_device)
+        want = paged.rope_append(q, kv, kv, k, v, slots + 8, slots, inv)
+        out.zero_()
+        assert torch.equal(paged.rope_append(src, kv, kv, k, v, slots + 8, slots, inv, q_out=out), want)
+        assert int((room != 0).sum()) <= out.numel()
