@@ -616,7 +616,9 @@ EXL3B200_API int exl3b200_rope_append(const exl3b200_rope_append_args* args, voi
  * device int32 [seqs], the new tokens included.  A length over max_pages * page_size (or over
  * 2^31 - 2049) is cut to it, a page id outside the pool reads as zeros; both record EXL3B200_EBADARG in the
  * device status.  A NaN or infinity in v at a position that one row of a sequence sees may
- * reach the sequence's other rows; beyond that nothing behind a mask is read.
+ * reach the sequence's other rows, an infinity also as NaN; beyond that nothing behind a mask
+ * is read.  Scores under -6.9e29 count as -inf, and a row of only those as one that sees
+ * nothing.  Weights are 16-bit pairs (2^-16 of their size), sums fp32, one rounding at the end.
  *
  * The sequences' lengths are read on the device: every CTA takes an equal run of the
  * batch's 64- or 128-position units, and a second kernel joins the sequences that the runs

@@ -20,12 +20,13 @@
 // again.  Elements are ordered by (value, lower index first) as unique 64-bit keys, so that
 // equal logits come in the order of their ids.
 //
-// Bound by HBM where rows are many: 2048 x 128256 bf16 (525 MB) take 92 us, 5.7 TB/s; what is
-// left is the exponential (16 a clock and SM, 60 us of it here) beside nearly seven other
-// instructions an element.  Whole rows to a CTA beat equal runs of units over all rows joined
-// by a second kernel (107 us; 500 x 151936 fp32: 57 instead of 77 us): a row's finish costs
-// more than an uneven last wave.  Few rows are a chain of latencies: 1 x 128256 9 us, 80 x
-// 151936 fp32 with 20 alternatives 18 us (48.6 MB).
+// Bound by HBM where rows are many: 2048 x 128256 bf16 (525 MB) take 92 us, 5.7 TB/s, in a
+// burst (a long run of calls settles at 102 to 106, 5 TB/s); what is left is the exponential
+// (16 a clock and SM, 60 us of it here) beside nearly seven other instructions an element.
+// Whole rows to a CTA beat equal runs of units over all rows joined by a second kernel (107
+// us; 500 x 151936 fp32: 57 instead of 77 us): a row's finish costs more than an uneven last
+// wave.  Few rows are a chain of latencies: 1 x 128256 9 us, 80 x 151936 fp32 with 20
+// alternatives 18 us (48.6 MB).
 #include <algorithm>
 #include <climits>
 
@@ -44,8 +45,12 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVec = 8;                       // elements of a thread's vector
 constexpr int kLpUnit = kLpThreads * kLpVec;    // elements of a unit
 constexpr int kLpCluster = 8;                   // most CTAs of a row
-// CTAs of a launch with clusters: 4 fit on an SM, but clusters do not pack a GPC's slots fully
-// (80 rows as clusters of 7, 95 % of the slots, took two waves: 27.5 us instead of 18.0 as 6)
+// CTAs of a launch with clusters: 4 fit on an SM, but clusters do not pack a GPC's slots
+// fully. 568 are resident as clusters of 8, 546 as 7, 558 to 568 as 3 to 6, 592 as pairs; 480
+// fit at every size, with rounding down to whole clusters counted.  80 rows of 151936 fp32 as
+// clusters of 7 (560 CTAs) took two waves: 27.5 us instead of 18.0 as 6; 80 of 128256 bf16
+// 20.3 instead of 14.2.  (Limits of 400 and 560 for 50 to 240 rows: up to 6 us slower at 400,
+// up to 3 faster at 560 where its clusters fit.)
 constexpr int kLpClusterCtas = 480;
 constexpr int kLpMaxTop = EXL3B200_LOGPROBS_MAX_TOP;
 constexpr int kLpBuffer = 1024;                 // candidates kept before they are cut back to the best 32

@@ -1264,7 +1264,7 @@ extern "C" int exl3b200_paged_attention(const exl3b200_paged_attention_args* p, 
     a.seqs = p->seqs, a.rows = p->rows_per_seq, a.group = p->q_heads / c.kv_heads, a.kv_heads = c.kv_heads;
     a.mblocks = sp.mblocks, a.mrows = sp.mrows, a.mtotal = sp.mtotal;
     a.page_size = c.page_size, a.num_pages = c.pages, a.capacity = (int) capacity;
-    // position / page_size as a multiplication (32-bit unsigned division by an invariant)
+    // position / page_size as a multiplication (unsigned division by an invariant, Granlund and Montgomery)
     int l = 0;
     while (l < 31 && (1u << l) < (unsigned) c.page_size) ++l;
     a.page_mul = (unsigned) ((((1ull << l) - (unsigned) c.page_size) << 32) / (unsigned) c.page_size + 1);
